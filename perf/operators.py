@@ -371,7 +371,7 @@ def _plain_attention(s):
 def _plain_sample(s):
     n, V = s["logits"].shape
     dev = s["logits"].device
-    col = lambda v: torch.as_tensor(v, device=dev).double().expand(n)[:, None]  # noqa: E731
+    col = lambda v: torch.as_tensor(v, device=dev, dtype=torch.float64).expand(n)[:, None]  # noqa: E731
     t, k, p, m, u = (col(s[x]) for x in ("temperature", "top_k", "top_p", "min_p", "u"))
     l = s["logits"].double()
     l = l.where(~l.isnan(), torch.full_like(l, float("-inf")))
@@ -504,7 +504,7 @@ def _exact_attention(s):
 def _exact_sample(s):
     """Row by row on the host, sums in extended precision."""
     n = s["logits"].shape[0]
-    par = {x: torch.as_tensor(s[x]).double().cpu().expand(n).numpy() for x in ("temperature", "top_k", "top_p", "min_p", "u")}
+    par = {x: torch.as_tensor(s[x], dtype=torch.float64).cpu().expand(n).numpy() for x in ("temperature", "top_k", "top_p", "min_p", "u")}
     logits = s["logits"].float().cpu().numpy()
     out = []
     for i in range(n):
