@@ -13,12 +13,13 @@ import torch
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libgdn_mi355x.so")
 
-F32, BF16, F16 = 0, 1, 2
+F32, BF16, F16, F8E4M3 = 0, 1, 2, 3
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _L = ctypes.c_int64
 _F = ctypes.c_float
+_D = ctypes.c_double
 
 _SIGNATURES = {
     "gdn_version": ([], _I),
@@ -68,6 +69,13 @@ _SIGNATURES = {
     "gdn_chunk_prefill_generic_workspace_bytes": ([_I, _I, _I, _I, _I], _L),
     "gdn_chunk_prefill_generic_ws": ([_P, _L, _P, _L, _P, _L, _P, _P, _I, _P, _P, _P, _I, _P, _L, _P, _I, _I, _I,
                                       _I, _I, _I, _I, _I, _P, _L, _P], _I),
+    "gdn_kv_store": ([_P, _L, _L, _P, _L, _L, _I, _P, _P, _P, _P, _I, _I, _I, _I, _L, _P, _P, _P, _I, _L, _P], _I),
+    "gdn_kv_load": ([_P, _P, _P, _P, _I, _I, _I, _I, _L, _P, _P, _P, _I, _L, _P, _P, _P], _I),
+    "gdn_attn_cached_workspace_bytes": ([_I, _I, _I, _I, _L, _I, _L], _L),
+    "gdn_attn_cached": ([_P, _L, _P, _I, _P, _P, _P, _P, _P, _P, _P, _P, _I, _L, _P, _P, _P, _P, _P, _P, _I, _L, _P, _L,
+                         _P, _L, _I, _I, _I, _I, _I, _F, _P], _I),
+    "gdn_sample_workspace_bytes": ([_I, _I], _L),
+    "gdn_sample": ([_P, _L, _I, _P, _I, _P, _P, _P, _P, _D, _I, _D, _D, _P, _I, _I, _P, _L, _P], _I),
 }
 
 _lib = None
@@ -113,6 +121,14 @@ def call(name, *args):
     if rc != 0:
         msg = lib().gdn_last_error().decode(errors="replace")
         raise GDNError(f"{name} failed (code {rc}): {msg}")
+
+
+def call_on(t, name, *args):
+    """``call`` with t's device as the current one (a launch goes to the current device's streams only)."""
+    if t.get_device() == torch.cuda.current_device():
+        return call(name, *args)
+    with torch.cuda.device(t.device):
+        return call(name, *args)
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)

@@ -14,7 +14,7 @@ OBJ = os.path.join(HERE, "_build")
 LIB_NAME = "libgdn_mi355x.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
 SOURCES = ["gdn_capi.hip", "gdn_decode.hip", "gdn_prefill.hip", "gdn_prefill_generic.hip", "gdn_gemv.hip",
-           "gdn_attn.hip"]
+           "gdn_attn.hip", "gdn_kv.hip", "gdn_attn_cached.hip", "gdn_sample.hip"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function",

@@ -24,6 +24,7 @@
 // ones, and P V multiplies those bf16 values against bf16 V with fp32 accumulation; the split's
 // exp-sum adds the same rounded values.  The test holds the result to an
 // fp32 reference.
+#include "gdn_attn.h"
 #include "gdn_device.h"
 #include "gdn_internal.h"
 
@@ -68,39 +69,6 @@ __host__ __device__ inline Work work_of(float* base, int N, int nh, int hd, int 
   w.o = reinterpret_cast<float*>(p);
   return w;
 }
-// The fused projection's row n, column col: a bf16 matrix, or bf16(sum of fp32 split-K partials
-// [splits][N][width] in split order) -- the same value the reduced projection holds.
-struct Src {
-  const uint16_t* bf;
-  int64_t stride;
-  const float* part;
-  int splits, N;
-  int64_t width;
-  __device__ __forceinline__ float operator()(int n, int64_t col) const {
-    if (!part) return bf2f(bf[n * stride + col]);
-    float s = 0.f;
-#pragma unroll 8
-    for (int sp = 0; sp < splits; ++sp) s += part[((int64_t)sp * N + n) * width + col];
-    return rbf(s);
-  }
-  // columns col + 64 e, the loads of several splits in flight
-  template <int E>
-  __device__ __forceinline__ void row(float (&x)[E], int n, int64_t col) const {
-    if (!part) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) x[e] = bf2f(bf[n * stride + col + 64 * e]);
-      return;
-    }
-#pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = 0.f;
-#pragma unroll 4
-    for (int sp = 0; sp < splits; ++sp)
-#pragma unroll
-      for (int e = 0; e < E; ++e) x[e] += part[((int64_t)sp * N + n) * width + col + 64 * e];
-#pragma unroll
-    for (int e = 0; e < E; ++e) x[e] = rbf(x[e]);
-  }
-};
 // Lane l's dims l + 64 e of a norm weight (as 1 + w) and, for dims below rd, of the rotary angle's frequency.
 template <int HD>
 struct NormRope {

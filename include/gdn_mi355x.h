@@ -7,8 +7,8 @@
  * allocates, never synchronises the host, and is therefore safe inside hipGraph stream capture.
  * Tensors are dense row-major unless a stride argument says otherwise; strides are in elements.
  *
- * Dtype codes: GDN_F32 = 0, GDN_BF16 = 1, GDN_F16 = 2 (IEEE half; taken by gdn_chunk_prefill_generic
- * only).  bf16 is stored as the upper 16 bits of an IEEE fp32.
+ * Dtype codes: GDN_F32 = 0, GDN_BF16 = 1, GDN_F16 = 2 (IEEE half; taken by gdn_chunk_prefill_generic,
+ * gdn_kv_store and gdn_sample only), GDN_F8E4M3 = 3 (OCP e4m3; a KV cache's dtype only).  bf16 is stored as the upper 16 bits of an IEEE fp32.
  * Return value: 0 on success, otherwise a GDN_E* code; gdn_last_error() then returns a message
  * (thread-local, valid until the next call on the same thread).
  *
@@ -25,7 +25,7 @@
 extern "C" {
 #endif
 
-enum { GDN_F32 = 0, GDN_BF16 = 1, GDN_F16 = 2 };
+enum { GDN_F32 = 0, GDN_BF16 = 1, GDN_F16 = 2, GDN_F8E4M3 = 3 };
 enum {
   GDN_OK = 0,
   GDN_EINVAL = 1,   /* bad shape, dtype, stride, alignment or null pointer */
@@ -451,6 +451,80 @@ int gdn_attn_decode_partial(const float* part, int splits, const int64_t* pos, c
                             const void* k_norm_w, const float* inv_freq, void* k_cache_t, void* v_cache, void* out,
                             int64_t out_stride, float* work, int64_t work_bytes, int N, int nh, int kv, int hd, int rd,
                             int T, float eps, void* stream);
+
+/*
+ * KV cache in bf16 or e4m3, filled from packed prompts and read by gdn_attn_cached.
+ *   Row r of R holds, for each of nkv heads, T tokens (T a multiple of 64) of hd values (64, 128 or 256):
+ *   k_cache, v_cache [R, nkv, T / 64, 64 * hd], 16-byte aligned, e4m3 codes or bf16.  A block's 64 tokens lie in the
+ *   order in which the attention reads them, in units of E values = 16 bytes (E = 16 in e4m3, 8 in bf16):
+ *     K: token 16 a + 4 i + r, dims E p .. E p + E - 1: unit ((p / 4 * 4 + i) * 4 + p % 4) * 16 + 4 a + r
+ *     V: dim 16 x + m, e4m3 tokens 16 a .. + 15: unit (16 x + m) * 4 + a;
+ *        bf16 tokens 16 a + 8 u .. + 7: unit ((2 x + u) * 16 + m) * 4 + a
+ *   k_exp, v_exp [R, nkv, T] (e4m3 only, 16-byte aligned): byte e + 127 of the row's scale 2^e: the value is code * 2^e.
+ *   e is the smallest integer >= -126 with max |x| <= 448 * 2^e over the row's finite values (0 for a row of zeros);
+ *   codes are rounded to nearest even; a value that is not finite becomes NaN.
+ * The batch: sequence s is the packed tokens cu_seqlens[s] .. cu_seqlens[s + 1] - 1 (device int32 [nseq + 1], or NULL for
+ * nseq equal lengths) and lies at positions start[s] + 0, 1, .. (device int32 [nseq], or NULL: 0) of cache row rows[s]
+ * (device int32 [nseq]).  No two sequences of a store may write the same position of the same row.
+ *   gdn_kv_store: K and V rows [total_tokens, nkv, hd] (in_dtype GDN_BF16, GDN_F16 or GDN_F32; token and head strides in
+ *     elements, rows of hd values 16-byte aligned) into the cache.  A row outside [0, R) or a position outside [0, T)
+ *     is not written; what no sequence covers stays as it was.
+ *   gdn_kv_load: out_k, out_v [total_tokens, nkv, hd] bf16 (dense, 16-byte aligned); rows and positions outside the cache
+ *     give zeros.
+ * Replaces the engine's copies of HF cache rows into its slots after a prefill (src/cb_engine.py:198-205, :229-239), and
+ * the prefill chunk's read of the slot's earlier keys and values.
+ */
+int gdn_kv_store(const void* xk, int64_t k_stride, int64_t k_head, const void* xv, int64_t v_stride, int64_t v_head,
+                 int in_dtype, void* k_cache, void* v_cache, uint8_t* k_exp, uint8_t* v_exp, int cache_dtype, int n_rows,
+                 int nkv, int hd, int64_t T, const int32_t* rows, const int32_t* cu_seqlens, const int32_t* start,
+                 int nseq, int64_t total_tokens, void* stream);
+int gdn_kv_load(const void* k_cache, const void* v_cache, const uint8_t* k_exp, const uint8_t* v_exp, int cache_dtype,
+                int n_rows, int nkv, int hd, int64_t T, const int32_t* rows, const int32_t* cu_seqlens,
+                const int32_t* start, int nseq, int64_t total_tokens, void* out_k, void* out_v, void* stream);
+
+/*
+ * gdn_attn_decode on such a cache (slot n is cache row n of N), optionally behind prefixes that slots share.
+ *   proj [N, proj_stride] bf16 as gdn_attn_decode, or (part not NULL) its split-K partial sums as
+ *     gdn_attn_decode_partial; pos, q_norm_w, k_norm_w, inv_freq, rd, out, out_stride, eps as there.
+ *   P prefixes (0: none): row r of the cache pre_k / pre_v / pre_k_exp / pre_v_exp (same dtype, heads and hd, Tp tokens)
+ *     holds positions 0 .. prefix_len[r] - 1 (device int32 [P], cut to [0, Tp]) for every slot with prefix_of[n] == r
+ *     (device int32 [N]; a value outside [0, P): no prefix).  The slot's own cache row then holds positions
+ *     prefix_len[r], .. from index 0 on: position pos[n] is written at index pos[n] - prefix_len[r].  Each prefix is read
+ *     once for all of its slots.
+ *   The new token attends to the whole prefix and to its own tokens up to itself.  A negative position writes nothing and
+ *   gives a zero output; one inside the prefix writes nothing and attends to the prefix alone; one behind the cache
+ *   row's end is not written and attends to all of the row.
+ *   work: gdn_attn_cached_workspace_bytes(N, nh, nkv, hd, T, P, Tp) bytes, 256-byte aligned (-1: bad sizes).
+ * hd in {64, 128, 256}; nh / nkv <= 16.  The query is rounded to bf16 once; scores, softmax and sums are fp32 (the
+ * probabilities enter P V as bf16); the rotary angle is formed in double.  Replaces CBEngine._attn's decode attention
+ * (src/cb_engine.py:265-276) on a cache of half the bytes.
+ */
+int64_t gdn_attn_cached_workspace_bytes(int N, int nh, int nkv, int hd, int64_t T, int P, int64_t Tp);
+int gdn_attn_cached(const void* proj, int64_t proj_stride, const float* part, int splits, const int64_t* pos,
+                    const void* q_norm_w, const void* k_norm_w, const float* inv_freq, void* k_cache, void* v_cache,
+                    uint8_t* k_exp, uint8_t* v_exp, int cache_dtype, int64_t T, const void* pre_k, const void* pre_v,
+                    const uint8_t* pre_k_exp, const uint8_t* pre_v_exp, const int32_t* prefix_len,
+                    const int32_t* prefix_of, int P, int64_t Tp, void* out, int64_t out_stride, void* work,
+                    int64_t work_bytes, int N, int nh, int nkv, int hd, int rd, float eps, void* stream);
+
+/*
+ * One token per row of logits [N, V] (dtype GDN_BF16, GDN_F16 or GDN_F32, row stride in elements).  With
+ * w_i = exp((l_i - max l) / temperature), kept are the top_k largest logits (<= 0 or >= V: all; ties: the lowest index),
+ * of these the fewest most likely ones whose mass reaches top_p of the top_k's mass (1: all; one at least), of these those
+ * with w_i >= min_p (the largest always); the token is the first index at which the kept weights' running sum exceeds
+ * u * their whole sum.  temperature <= 0 (or NaN): the first index of the maximum.  Logits of -inf or NaN are never
+ * taken; a row that has nothing else gives -1.
+ *   u [N] fp32 (or fp64 with u_is_f64) in [0, 1) on the device (values outside are cut to it).
+ *   temperature, top_k, top_p, min_p: per row [N] on the device (fp32, int32, fp32, fp32), or NULL and the value *1 for
+ *     every row.  out [N] int64.
+ *   work: gdn_sample_workspace_bytes(N, V) bytes, 256-byte aligned; its contents need no clearing.
+ * Weights and sums are 64-bit, and sums do not depend on an order: the same inputs give the same token.  Replaces the
+ * argmax over the engine's logits (src/cb_engine.py:170-172).
+ */
+int64_t gdn_sample_workspace_bytes(int N, int V);
+int gdn_sample(const void* logits, int64_t stride, int dtype, const void* u, int u_is_f64, const float* temperature,
+               const int32_t* top_k, const float* top_p, const float* min_p, double temperature1, int top_k1, double top_p1,
+               double min_p1, int64_t* out, int N, int V, void* work, int64_t work_bytes, void* stream);
 
 #ifdef __cplusplus
 }
