@@ -24,7 +24,7 @@ constexpr int CHUNK = TH * EPT;   // a row's elements per workgroup
 constexpr int NW = TH / 64, WAVE = 64 * EPT;  // its waves, and their elements
 constexpr int BINS = 256;         // of a digit
 constexpr int COLS = 16;          // a bin's counters in LDS
-constexpr int DT = 256;           // threads of the draw
+constexpr int DT = 512;           // threads of the draw
 constexpr int MOST = 1024 * CHUNK;  // logits of a row (the draw keeps its chunks in LDS)
 typedef unsigned long long u64;
 
@@ -61,6 +61,7 @@ struct State {
   double target;    // top_p: the mass to reach
   int32_t left;     // top_k: the rank still to find in the bin
   int32_t quota;    // -1: no cut
+  int after_k;      // top_p's descent, behind top_k's
   uint32_t thr;     // the cut so far: keys above thr are kept, and the first `quota` elements with key thr
 };
 struct Hist {  // [N][S][BINS]
@@ -71,7 +72,7 @@ struct Work {
   float* lmax;      // [N][S]: the chunks' maxima and their first indexes
   int32_t* larg;
   State* state;     // [2][N]
-  Hist first, step[2];
+  Hist step[7];     // pass i's
   int64_t* kept;    // [N][S][NW]: mass above the cut and elements at it, of each wave's elements
   int32_t* ties;
 };
@@ -201,6 +202,7 @@ template <int W> struct Scratch {
   uint32_t count[W][BINS];  // each wave's share of the chunks
   double mass[W][BINS];
   State st;
+  double w;
 };
 // One digit: the row's chunks merged, and by the first wave the bin in which the cut lies (sc.st).  root: the descent's
 // first digit, whose masses are relative to the chunks' own maxima (top_p: of mass, its target's base; below 0: the row's
@@ -217,7 +219,7 @@ __device__ __forceinline__ void choose(const Hist& h, bool root, const Work& wk,
   const uint32_t* hc = h.count + (int64_t)n * S * BINS + 4 * lane;
   const u64* hm = h.mass + (int64_t)n * S * BINS + 4 * lane;
   if (weigh) {
-#pragma unroll 4
+#pragma unroll 2
     for (int s = wid; s < S; s += W) {
       const uint4 c1 = *reinterpret_cast<const uint4*>(hc + (int64_t)s * BINS);
       const ulonglong2 m0 = *reinterpret_cast<const ulonglong2*>(hm + (int64_t)s * BINS);
@@ -228,7 +230,7 @@ __device__ __forceinline__ void choose(const Hist& h, bool root, const Work& wk,
       m[2] = fma((double)m1.x, f, m[2]), m[3] = fma((double)m1.y, f, m[3]);
     }
   } else {
-#pragma unroll 4
+#pragma unroll 2
     for (int s = wid; s < S; s += W) {
       const uint4 c1 = *reinterpret_cast<const uint4*>(hc + (int64_t)s * BINS);
       c[0] += c1.x, c[1] += c1.y, c[2] += c1.z, c[3] += c1.w;
@@ -293,57 +295,67 @@ __device__ __forceinline__ void choose(const Hist& h, bool root, const Work& wk,
       if (hits) hits &= -hits;
     }
     if (hits && lane == 63 - __builtin_clzll(hits)) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (e == hit) {
-          st.left -= (int)cs[e];
-          st.above += ms[e];
-          st.prefix = st.prefix << 8 | (uint32_t)(4 * lane + e);
-          ++st.level;
-          sc.st = st;
-          sc.mass[0][0] = v[e];
-        }
+      st.left -= (int)(hit == 0 ? cs[0] : hit == 1 ? cs[1] : hit == 2 ? cs[2] : cs[3]);
+      st.above += hit == 0 ? ms[0] : hit == 1 ? ms[1] : hit == 2 ? ms[2] : ms[3];
+      st.prefix = st.prefix << 8 | (uint32_t)(4 * lane + hit);
+      ++st.level;
+      sc.st = st;
+      sc.w = hit == 0 ? v[0] : hit == 1 ? v[1] : hit == 2 ? v[2] : v[3];
     }
   }
   __syncthreads();
-  w = sc.mass[0][0];
+  w = sc.w;
 }
 // The row's state (sc.st) at the beginning of pass i >= 1 (or of the draw, i = the passes' number), from the state at the
-// beginning of pass i - 1 and that pass's histogram.  Barriers in it; one at its end.
+// beginning of pass i - 1 and that pass's histogram.  top_k's descent has had the passes 0 .. levels - 1 in turn; top_p's,
+// which follows it, takes the same histograms as long as its digits are the same.  Barriers in it; one at its end.
 template <int W>
 __device__ __forceinline__ void advance(const Job& J, const Work& wk, const Row& r, int n, int i, const double* table,
                                         Scratch<W>& sc) {
   const bool root = i == 1;
-  if (threadIdx.x < 64) {
-    State st{};
-    if (root) {
-      float m = -INFINITY;
-      for (int s = threadIdx.x; s < J.S; s += 64) m = fmaxf(m, wk.lmax[(int64_t)n * J.S + s]);
-      st.M = wave_max_fast(m);
-      st.quota = -1;
-      if (!r.greedy && st.M != -INFINITY) st.kind = r.by_k ? 1 : r.by_p ? 2 : 0;
-      st.left = r.k;
-    } else {
-      st = wk.state[(int64_t)((i - 1) & 1) * J.N + n];
+  if (!root) {
+    // (a word a lane)
+    const uint32_t* from = reinterpret_cast<const uint32_t*>(wk.state + (int64_t)((i - 1) & 1) * J.N + n);
+    if (threadIdx.x < sizeof(State) / 4) reinterpret_cast<uint32_t*>(&sc.st)[threadIdx.x] = from[threadIdx.x];
+  } else if (threadIdx.x < 64) {
+    float m = -INFINITY;
+    for (int s = threadIdx.x; s < J.S; s += 64) m = fmaxf(m, wk.lmax[(int64_t)n * J.S + s]);
+    m = wave_max_fast(m);
+    if (threadIdx.x == 0) {
+      sc.st.M = m;
+      sc.st.kind = r.greedy || m == -INFINITY ? 0 : r.by_k ? 1 : r.by_p ? 2 : 0;
+      sc.st.level = 0;
+      sc.st.prefix = 0;
+      sc.st.above = 0;
+      sc.st.target = 0;
+      sc.st.left = r.k;
+      sc.st.quota = -1;
+      sc.st.after_k = 0;
+      sc.st.thr = 0;
     }
-    if (threadIdx.x == 0) sc.st = st;
   }
   __syncthreads();
   if (!sc.st.kind) return;
   const Weights wt(r.t, sc.st.M, table);
   double base = -1.0, w;
-  for (bool first = root;; first = true) {  // twice where top_k's descent ends here and top_p's begins
-    choose(first ? wk.first : wk.step[(i - 1) & 1], first, wk, r, wt, n, J.S, J.levels, sc, base, w);
-    if (sc.st.level < J.levels) return;
+  for (int h = i - 1;;) {
+    choose(wk.step[h], h == 0, wk, r, wt, n, J.S, J.levels, sc, base, w);
     State st = sc.st;
+    if (st.level < J.levels) {
+      if (!st.after_k || st.thr >> (32 - 8 * st.level - (32 - 8 * J.levels)) != st.prefix) return;
+      ++h;  // top_p's descent along top_k's
+      continue;
+    }
     if (st.kind == 1) {
       st.thr = st.prefix;
       st.quota = st.left;
       base = st.above + (double)st.quota * w;
       st.kind = r.by_p ? 2 : 0;
+      st.after_k = r.by_p;
       st.level = 0;
       st.prefix = 0;
       st.above = 0;
+      h = 0;
     } else {
       const double m = ceil((st.target - st.above) / w);
       const int32_t q = m >= 1.0 ? m < 2e9 ? (int32_t)m : INT32_MAX : 1;
@@ -359,22 +371,43 @@ __device__ __forceinline__ void advance(const Job& J, const Work& wk, const Row&
 }
 }  // namespace sample
 
-// Pass i of `passes`, grid (S, N): the histogram of the next digit of the elements whose earlier digits are the prefix (pass
-// 0: of all), and in the last pass each wave's mass above the prefix, or above the cut and the elements at it where that is
-// known.
-//
-// A wave's values crowd a few bins, and a counter in LDS takes one lane's addition at a time: each bin has COLS counters,
-// lane l adding to the (l % COLS)-th.  (One counter a bin and wave: 30 us for 61 workgroups of 4096 logits.)
+// Elements into a histogram, in LDS.  A wave's values crowd a few bins, and a counter takes one lane's addition at a time:
+// each bin has COLS counters, lane l adding to the (l % COLS)-th.  (One counter a bin and wave: 30 us for 61 workgroups of
+// 4096 logits.)
+namespace sample {
+struct Counters {
+  u64 mass[BINS * COLS];
+  uint32_t count[BINS * COLS];
+  __device__ __forceinline__ void clear() {  // (and a barrier)
+    for (int x = threadIdx.x; x < (int)sizeof(Counters) / 16; x += TH) reinterpret_cast<uint4*>(this)[x] = uint4{0, 0, 0, 0};
+  }
+  // TH / BINS threads a bin; they begin at different counters, so that a wave's reads spread over the banks
+  __device__ __forceinline__ void write(const Hist& h, int64_t at, bool weigh) const {
+    constexpr int PER = TH / BINS;
+    const int tid = threadIdx.x, bin = tid / PER;
+    uint32_t a = 0;
+    u64 m = 0;
+#pragma unroll
+    for (int x = 0; x < COLS / PER; ++x) {
+      const int col = bin * COLS + tid % PER * (COLS / PER) + (x + bin) % (COLS / PER);
+      a += count[col];
+      if (weigh) m += mass[col];
+    }
+#pragma unroll
+    for (int o = 1; o < PER; o <<= 1) a += __shfl_xor(a, o, kWave), m += __shfl_xor(m, o, kWave);
+    if (tid % PER == 0) {
+      h.count[at * BINS + bin] = a;
+      h.mass[at * BINS + bin] = m;
+    }
+  }
+};
+}  // namespace sample
+
+// Pass 0, grid (S, N): the chunks' maxima, and the histogram of the first digit.
 template <typename T>
-__global__ __launch_bounds__(sample::TH) void sample_pass_kernel(sample::Job J, sample::Work wk, int i, int passes) {
+__global__ __launch_bounds__(sample::TH, 4) void sample_first_kernel(sample::Job J, sample::Work wk) {
   using namespace sample;
-  __shared__ union {
-    Scratch<NW> sc;
-    struct {
-      u64 mass[BINS * COLS];
-      uint32_t count[BINS * COLS];
-    } h;
-  } lds;
+  __shared__ Counters lds;
   __shared__ double table[64];
   __shared__ float tf[NW];
   __shared__ int first;
@@ -383,45 +416,71 @@ __global__ __launch_bounds__(sample::TH) void sample_pass_kernel(sample::Job J, 
   Chunk<T, EPT> c;
   c.load(static_cast<const T*>(J.logits) + n * J.stride, (int64_t)s * CHUNK + wid * WAVE, J.V);
   const Row r = row_of(J.par, n, J.V);
+  const bool count = !r.greedy && (r.by_k || r.by_p);
   if (tid < 64) table[tid] = kPow[tid];
-  State st{};
+  if (tid == 0) first = CHUNK;
+  if (count) lds.clear();
   float M = -INFINITY;
-  if (i == 0) {
-    int arg = 0;
+  int arg = 0;
 #pragma unroll
-    for (int e = 0; e < EPT; ++e)
-      if (c[e] > M) M = c[e], arg = wid * WAVE + Chunk<T, EPT>::index(e);  // a thread's indexes ascend
-    const float mine = M;
-    M = wave_max_fast(M);
-    if (lane == 0) tf[wid] = M;
-    if (tid == 0) first = CHUNK;
-    __syncthreads();
+  for (int e = 0; e < EPT; ++e)
+    if (c[e] > M) M = c[e], arg = wid * WAVE + Chunk<T, EPT>::index(e);  // a thread's indexes ascend
+  const float mine = M;
+  M = wave_max_fast(M);
+  if (lane == 0) tf[wid] = M;
+  __syncthreads();
 #pragma unroll
-    for (int w = 0; w < NW; ++w) M = fmaxf(M, tf[w]);
-    if (mine == M) atomicMin(&first, arg);
-    __syncthreads();
-    if (tid == 0) {
-      wk.lmax[at] = M;
-      wk.larg[at] = s * CHUNK + first;
-    }
-    if (r.greedy || !(r.by_k || r.by_p)) return;
-  } else {
-    advance(J, wk, r, n, i, table, lds.sc);
-    st = lds.sc.st;
-    if (s == 0 && tid == 0) wk.state[(int64_t)(i & 1) * J.N + n] = st;
-    if (r.greedy || st.M == -INFINITY || (!st.kind && i < passes - 1)) return;
-    M = st.M;
-    __syncthreads();
-  }
-  const bool last = i && i == passes - 1, count = i == 0 || st.kind;
-  const bool weigh = count && r.by_p && M != -INFINITY && st.level < J.levels - 1;
-  const bool tally = count && (r.by_k || i);  // top_p's first digit goes by mass alone
+  for (int w = 0; w < NW; ++w) M = fmaxf(M, tf[w]);
+  if (mine == M) atomicMin(&first, arg);
   if (count) {
-    for (int x = tid; x < (int)sizeof(lds.h) / 16; x += TH) reinterpret_cast<uint4*>(&lds.h)[x] = uint4{0, 0, 0, 0};
+    const Weights wt(r.t, M, table);
+    const bool weigh = r.by_p && M != -INFINITY;
+#pragma unroll
+    for (int e = 0; e < EPT; ++e) {
+      const float v = c[e];
+      const int b = (key_of(v) >> 24) * COLS + tid % COLS;
+      if (r.by_k) atomicAdd(&lds.count[b], 1u);  // (top_p's first digit goes by mass alone)
+      if (weigh) atomicAdd(&lds.mass[b], fixed(wt(v), 0x1p50));
+    }
+  }
+  __syncthreads();
+  if (tid == 0) {
+    wk.lmax[at] = M;
+    wk.larg[at] = s * CHUNK + first;
+  }
+  if (count) lds.write(wk.step[0], at, r.by_p);
+}
+
+// Pass i >= 1 of `passes`, grid (S, N): the histogram of the next digit of the elements whose earlier digits are the prefix,
+// and in the last pass each wave's mass above the prefix, or above the cut and the elements at it where that is known.
+template <typename T>
+__global__ __launch_bounds__(sample::TH, 4) void sample_pass_kernel(sample::Job J, sample::Work wk, int i, int passes) {
+  using namespace sample;
+  __shared__ union {
+    Scratch<NW> sc;
+    Counters h;
+  } lds;
+  __shared__ double table[64];
+  const int n = blockIdx.y, s = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+  const int64_t at = (int64_t)n * J.S + s;
+  Chunk<T, EPT> c;
+  c.load(static_cast<const T*>(J.logits) + n * J.stride, (int64_t)s * CHUNK + wid * WAVE, J.V);
+  const Row r = row_of(J.par, n, J.V);
+  if (tid < 64) table[tid] = kPow[tid];
+  advance(J, wk, r, n, i, table, lds.sc);
+  const State st = lds.sc.st;
+  if (s == 0 && tid < (int)sizeof(State) / 4)
+    reinterpret_cast<uint32_t*>(wk.state + (int64_t)(i & 1) * J.N + n)[tid] = reinterpret_cast<const uint32_t*>(&lds.sc.st)[tid];
+  const bool last = i == passes - 1, count = st.kind;
+  if (r.greedy || st.M == -INFINITY || !(count || last)) return;
+  __syncthreads();
+  const bool weigh = count && r.by_p && st.level < J.levels - 1;
+  if (count) {
+    lds.h.clear();
     __syncthreads();
   }
   // keys are compared up to the digits known: the prefix, or the whole cut (no cut: every key of a number is above 0)
-  const Weights wt(r.t, M, table);
+  const Weights wt(r.t, st.M, table);
   const int dsh = 24 - 8 * st.level, sh = count ? dsh + 8 : 32 - 8 * J.levels;
   const uint32_t ref = count ? st.prefix : st.quota >= 0 ? st.thr : 0;
   int64_t mass = 0;
@@ -429,18 +488,17 @@ __global__ __launch_bounds__(sample::TH) void sample_pass_kernel(sample::Job J, 
 #pragma unroll
   for (int e = 0; e < EPT; ++e) {
     const float v = c[e];
-    const uint32_t k = key_of(v);
-    const uint32_t k1 = sh < 32 ? k >> sh : 0;
+    const uint32_t k = key_of(v), k1 = k >> sh;
     const bool in = k1 == ref, above = last && k1 > ref && v != -INFINITY;
     u64 w = 0;
     if (above || (in && weigh)) {
       const double x = wt(v);
       w = fixed(x, above ? J.one : 0x1p50);
-      if (above && (x >= r.m || v == M)) mass += (int64_t)w;
+      if (above && (x >= r.m || v == st.M)) mass += (int64_t)w;
     }
     if (in && count) {
       const int b = (k >> dsh & 255u) * COLS + tid % COLS;
-      if (tally) atomicAdd(&lds.h.count[b], 1u);
+      atomicAdd(&lds.h.count[b], 1u);
       if (weigh) atomicAdd(&lds.h.mass[b], w);
     }
     ties += in;
@@ -455,24 +513,7 @@ __global__ __launch_bounds__(sample::TH) void sample_pass_kernel(sample::Job J, 
   }
   if (!count) return;
   __syncthreads();
-  // TH / BINS threads a bin; they begin at different counters, so that a wave's reads spread over the banks
-  constexpr int PER = TH / BINS;
-  const Hist& h = i == 0 ? wk.first : wk.step[i & 1];
-  const int bin = tid / PER;
-  uint32_t a = 0;
-  u64 m = 0;
-#pragma unroll
-  for (int x = 0; x < COLS / PER; ++x) {
-    const int col = bin * COLS + tid % PER * (COLS / PER) + (x + bin) % (COLS / PER);
-    a += lds.h.count[col];
-    if (weigh) m += lds.h.mass[col];
-  }
-#pragma unroll
-  for (int o = 1; o < PER; o <<= 1) a += __shfl_xor(a, o, kWave), m += __shfl_xor(m, o, kWave);
-  if (tid % PER == 0) {
-    h.count[at * BINS + bin] = a;
-    h.mass[at * BINS + bin] = m;
-  }
+  lds.h.write(wk.step[i], at, weigh);
 }
 
 // grid (N): the draw.  Sums of weights are whole numbers here: first over chunks, then over the found chunk's waves, then
@@ -509,14 +550,14 @@ __global__ __launch_bounds__(sample::DT) void sample_draw_kernel(sample::Job J, 
   const uint32_t digit = st.thr & 255u;
   const int64_t quota = cut ? st.quota : 0;
   // an element's mass by its last digit (0: min_p drops it), at the cut and above it
-  {
+  if (tid < BINS) {
     const float v = value_of((cut ? st.thr & ~255u : 0u) | (uint32_t)tid, J.levels);
     const double w = weight(v);
     bin_mass[tid] = cut && (uint32_t)tid >= digit && v <= st.M && (w >= r.m || v == st.M) ? (int64_t)fixed(w, J.one) : 0;
   }
   __syncthreads();
   const int64_t wt = cut ? bin_mass[digit] : 0;
-  const uint32_t* count = wk.step[(passes - 1) & 1].count;
+  const uint32_t* count = wk.step[passes - 1].count;
   for (int s = wid; s < J.S; s += W) {
     int64_t m = lane < NW ? wk.kept[(base + s) * NW + lane] : 0;
     int t = lane < NW && !open ? wk.ties[(base + s) * NW + lane] : 0;
@@ -643,7 +684,8 @@ template <typename T>
 static int launch_sample(sample::Job J, const sample::Work& wk, bool by_k, bool by_p, hipStream_t st) {
   const dim3 g(J.S, J.N);
   const int open = ((int)by_k + (int)by_p) * (J.levels - 1), passes = 1 + (open ? open : 1);
-  for (int i = 0; i < passes; ++i) sample_pass_kernel<T><<<g, sample::TH, 0, st>>>(J, wk, i, passes);
+  sample_first_kernel<T><<<g, sample::TH, 0, st>>>(J, wk);
+  for (int i = 1; i < passes; ++i) sample_pass_kernel<T><<<g, sample::TH, 0, st>>>(J, wk, i, passes);
   sample_draw_kernel<T><<<J.N, sample::DT, 0, st>>>(J, wk, passes);
   return check_launch("gdn_sample");
 }
@@ -665,9 +707,9 @@ int64_t sample_work(sample::Work& w, char* p, int N, int V) {
   w.state = reinterpret_cast<sample::State*>(take(2ll * N * sizeof(sample::State)));
   w.kept = reinterpret_cast<int64_t*>(take(items * sample::NW * 8));
   w.ties = reinterpret_cast<int32_t*>(take(items * sample::NW * 4));
-  for (sample::Hist* h : {&w.first, &w.step[0], &w.step[1]}) {
-    h->mass = reinterpret_cast<sample::u64*>(take(items * sample::BINS * 8));
-    h->count = reinterpret_cast<uint32_t*>(take(items * sample::BINS * 4));
+  for (sample::Hist& h : w.step) {
+    h.mass = reinterpret_cast<sample::u64*>(take(items * sample::BINS * 8));
+    h.count = reinterpret_cast<uint32_t*>(take(items * sample::BINS * 4));
   }
   return p - base;
 }
