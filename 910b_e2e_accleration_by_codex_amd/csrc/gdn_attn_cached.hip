@@ -6,14 +6,15 @@
 //   o = sum_t p_t v_t / sum_t p_t, p_t = exp(q . k_t / sqrt(hd)), over the slot's prefix and its own tokens;
 //   out = o sigmoid(gate).
 // Launches:
-//   1. cached_prep_kernel: a wave per (slot, head row).  Norm, rotary (angles in double), q as bf16 to the workspace, k and
+//   1. cached_prep_kernel: a wave per (slot, head row).  Norm, rotary (angles in double), q to the workspace, k and
 //      v quantised into the cache.  One more workgroup sorts the slots by prefix into tiles of 32 query rows.
 //   2. cached_split_kernel: partial softmax sums of a range of tokens for 16 query rows (the G heads of one slot's kv
 //      head) or 32 (a tile of a prefix's slots).
 //   3. cached_combine_kernel: per (slot, head) the partials merged by their maxima, and the gate.
-// Rounding: q once to bf16 (an MFMA operand); K and V enter as the cache holds them (e4m3 codes are bf16 values, their
-// scales multiply scores and probabilities in fp32); scores, maxima, sums and outputs fp32; probabilities (times V's
-// scale) to bf16, their sum adds the same rounded values; the output once to bf16.
+// Rounding: K and V enter as the cache holds them (e4m3 codes are bf16 values, their scales multiply scores and
+// probabilities in fp32).  The query and the probabilities are fp32 values that enter the bf16 products as a high and a low
+// part, two products each: one rounding of each to bf16 would nearly double the error of the rounded output (0.0031
+// against 0.0017 relative), and these products are not what bounds the kernel.  The output is rounded once, to bf16.
 #include "gdn_attn.h"
 #include "gdn_device.h"
 #include "gdn_internal.h"
@@ -35,9 +36,37 @@ __device__ __forceinline__ u32x4 widen(uint32_t lo, uint32_t hi) {
                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false)),
                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true))};
 }
+// A value as the sum of two bf16: the upper half of it, cut off (two values paired), and what is left.  Both parts have the
+// value's sign, and against a bf16 cache, which may hold infinities, a low part of a value is never 0: times an infinity
+// the parts' products are that infinity twice, as the value's is.
+__device__ __forceinline__ uint32_t high2(float a, float b) {
+  return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+}
+template <bool F8> __device__ __forceinline__ float low(float x) {  // x >= 0
+  const float r = x - __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+  return F8 ? r : fmaxf(r, x > 0.f ? 0x1p-126f : 0.f);
+}
+// The registers' values are not needed any more: without this, a load that only one branch does keeps the other branch's old
+// values alive.
+template <int N> __device__ __forceinline__ void drop(u32x4 (&x)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "=v"(x[i]));
+}
 constexpr int WAVES = 4;       // per split workgroup; a wave takes every 4th block of the range
 constexpr int PROWS = 32;      // query rows of a prefix tile
 
+// Ranges that a row of up to T tokens is cut into (parts at most), of `least` blocks at least: a block per wave where a
+// workgroup for each such range finds room on the chip at once (one fits a CU), else two, and about 4 workgroups a CU
+// where rows are long.
+struct Cut {
+  int parts, least;
+};
+inline Cut cut_of(int64_t T, int64_t items) {
+  const int64_t n = (T + BT - 1) / BT, four = (n + WAVES - 1) / WAVES;
+  const int least = four * items <= 256 ? WAVES : 2 * WAVES;
+  const int64_t most = (n + least - 1) / least, want = (1024 + items - 1) / items;
+  return Cut{(int)(most < want ? most : want), least};
+}
 struct Side {  // one cache: its tensors and its length (tokens, a multiple of 64)
   uint8_t *k, *v, *ke, *ve;
   int64_t T;
@@ -50,16 +79,15 @@ struct Args {
   Side own, pre;
   const int32_t *plen, *pof;  // NULL: no prefixes
   int N, nh, nkv, rd, P, tiles;
-  int S, SP;  // partials per head: of the slot's own tokens, of its prefix
+  Cut S, SP;  // partials per head: of the slot's own tokens, of its prefix
   float eps;
   uint16_t* out;
   int64_t out_stride;
 };
-// workspace: q (bf16 [N, nh, hd]) | m, l (fp32 [N, nh, S + SP, 2]) | o (fp32 [N, nh, S + SP, hd]) | order (int32 [N]) |
+// workspace: q (fp32 [N, nh, hd]) | m, l (fp32 [N, nh, S + SP, 2]) | o (fp32 [N, nh, S + SP, hd]) | order (int32 [N]) |
 // tiles (int32 [tiles, 4]: prefix, its first place in order, first row, rows)
 struct Work {
-  uint16_t* q;
-  float *ml, *o;
+  float *q, *ml, *o;
   int32_t* order;
   int4* tiles;
 };
@@ -71,8 +99,8 @@ inline int most_tiles(int N, int G, int P) {  // a prefix of m slots has ceil(m 
 __host__ __device__ inline int64_t round256(int64_t b) { return (b + 255) / 256 * 256; }
 inline int64_t work_of(Work& w, char* p, int N, int nh, int nkv, int hd, int parts, int P) {
   char* const base = p;
-  w.q = reinterpret_cast<uint16_t*>(p);
-  p += round256((int64_t)N * nh * hd * 2);
+  w.q = reinterpret_cast<float*>(p);
+  p += round256((int64_t)N * nh * hd * 4);
   w.ml = reinterpret_cast<float*>(p);
   p += round256((int64_t)N * nh * parts * 8);
   w.o = reinterpret_cast<float*>(p);
@@ -82,11 +110,6 @@ inline int64_t work_of(Work& w, char* p, int N, int nh, int nkv, int hd, int par
   w.tiles = reinterpret_cast<int4*>(p);
   p += P ? round256((int64_t)most_tiles(N, nh / nkv, P) * 16) : 0;
   return p - base;
-}
-// Ranges a row of T tokens is cut into: at least 256 tokens each (a block per wave), and about 2048 workgroups in all.
-inline int parts_of(int64_t T, int64_t items) {
-  const int64_t most = (T + 255) / 256, want = (2048 + items - 1) / items;
-  return (int)(most < want ? most : want);
 }
 // What a slot attends to.
 struct Slot {
@@ -109,14 +132,14 @@ __device__ __forceinline__ Slot slot_of(const Args& A, int n) {
   s.at = at < A.own.T ? at : -1;
   return s;
 }
-// Blocks per range when n blocks go to at most `parts` ranges, 4 at least (one per wave).
-__device__ __forceinline__ int64_t range_blocks(int64_t n, int parts) {
-  const int64_t b = (n + parts - 1) / parts;
-  return b < WAVES ? WAVES : b;
+// Blocks per range of n blocks.
+__device__ __forceinline__ int64_t range_blocks(int64_t n, const Cut& c) {
+  const int64_t b = (n + c.parts - 1) / c.parts;
+  return b < c.least ? c.least : b;
 }
-__device__ __forceinline__ int ranges(int64_t tokens, int parts) {
+__device__ __forceinline__ int ranges(int64_t tokens, const Cut& c) {
   const int64_t n = (tokens + BT - 1) / BT;
-  const int64_t b = range_blocks(n, parts);
+  const int64_t b = range_blocks(n, c);
   return (int)((n + b - 1) / b);
 }
 }  // namespace cached
@@ -190,7 +213,7 @@ __global__ __launch_bounds__(256) void cached_prep_kernel(cached::Args A, cached
   }
   if (is_q) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) wk.q[((int64_t)n * A.nh + r) * HD + lane + 64 * e] = f2bf(x[e]);
+    for (int e = 0; e < E; ++e) wk.q[((int64_t)n * A.nh + r) * HD + lane + 64 * e] = x[e];
     return;
   }
   const int64_t row = ((int64_t)n * A.nkv + j) * A.own.T;
@@ -224,12 +247,12 @@ __global__ __launch_bounds__(256) void cached_prep_kernel(cached::Args A, cached
 //      for token 16 g + 8 u + e: the lane's own scores are its operand.  O's lane (c, g) has row c, dims 16 x + 4 g + r, so
 //      the running maximum's corrections are a number per lane.
 template <int HD, bool F8, int RT>
-__global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void cached_split_kernel(cached::Args A, cached::Work wk, float scale2) {
+__global__ __launch_bounds__(256, RT == 1 && HD < 256 ? 2 : 1) void cached_split_kernel(cached::Args A, cached::Work wk, float scale2) {
   using namespace cached;
   constexpr int R = 16 * RT, LQ = HD + 8;
   constexpr int KS = HD / 32, X = HD / 16;  // 32-dim steps of the scores, 16-dim tiles of the output
   constexpr int DS = 64;                    // dims per round of the merge
-  __shared__ alignas(16) uint16_t qs[R * LQ];
+  __shared__ alignas(16) uint16_t qs[2][R * LQ];
   __shared__ alignas(16) float so[WAVES][R][DS + 4];
   __shared__ float sm[WAVES][R], sl[WAVES][R];
   __shared__ int rown[R], rowh[R];  // each row's slot (-1: none) and head
@@ -238,7 +261,7 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void cached_split_kernel(cach
   const int part = blockIdx.x, j = blockIdx.y, G = A.nh / A.nkv;
   int64_t tokens, row;  // of the cache row
   const Side& side = RT == 1 ? A.own : A.pre;
-  const int parts = RT == 1 ? A.S : A.SP;
+  const Cut& cut = RT == 1 ? A.S : A.SP;
   if (RT == 1) {
     const int n = blockIdx.z;
     tokens = slot_of(A, n).own;
@@ -258,21 +281,31 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void cached_split_kernel(cach
       rowh[tid] = j * G + q % G;
     }
   }
-  const int64_t nblk = (tokens + BT - 1) / BT, per = range_blocks(nblk, parts);
+  const int64_t nblk = (tokens + BT - 1) / BT, per = range_blocks(nblk, cut);
   const int64_t b0 = part * per, b1 = b0 + per < nblk ? b0 + per : nblk;
   if (b0 >= b1) return;
-  __syncthreads();
-  for (int i = tid; i < R * (HD / 8); i += 64 * WAVES) {
-    const int q = i / (HD / 8), d = 8 * (i % (HD / 8));
-    u32x4 v = {0, 0, 0, 0};
-    if (rown[q] >= 0) v = *reinterpret_cast<const u32x4*>(&wk.q[((int64_t)rown[q] * A.nh + rowh[q]) * HD + d]);
-    *reinterpret_cast<u32x4*>(&qs[q * LQ + d]) = v;
-  }
-  __syncthreads();
+  lds_barrier();
   constexpr int S1 = F8 ? 1 : 2;
+  constexpr int KL = HD / 16 * S1, VL = X * S1;  // 16-byte loads of a block's K and V, per lane
+  // Loads ahead: the next block's K goes out when this one's scores are done, its V when this one's is used up.
   const int64_t hrow = (row * A.nkv + j) * side.T;
   const uint8_t* kp = side.k + hrow * HD * S1;
   const uint8_t* vp = side.v + hrow * HD * S1;
+  const int kat = lane * 16, vat = c * 64 + g * 16;
+  u32x4 kr[KL], vr[VL], kx = {0, 0, 0, 0}, vx = {0, 0, 0, 0};
+  // (buffer loads: the block's address is scalar, a lane's offset one register for all of them)
+  auto load_k = [&](int64_t b) {
+    if constexpr (F8) kx = *reinterpret_cast<const u32x4*>(side.ke + hrow + b * BT + 16 * g);
+    const auto block = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(kp) + b * (BT * HD * S1), 0, BT * HD * S1, 0x00027000);
+#pragma unroll
+    for (int i = 0; i < KL; ++i) kr[i] = __builtin_amdgcn_raw_buffer_load_b128(block, kat, i * 1024, 0);
+  };
+  auto load_v = [&](int64_t b) {
+    if constexpr (F8) vx = *reinterpret_cast<const u32x4*>(side.ve + hrow + b * BT + 16 * g);
+    const auto block = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(vp) + b * (BT * HD * S1), 0, BT * HD * S1, 0x00027000);
+#pragma unroll
+    for (int i = 0; i < VL; ++i) vr[i] = __builtin_amdgcn_raw_buffer_load_b128(block, vat, i * 1024, 0);
+  };
   float m[RT], l[RT];
   f32x4 O[RT][X];
 #pragma unroll
@@ -282,42 +315,71 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void cached_split_kernel(cach
 #pragma unroll
     for (int x = 0; x < X; ++x) O[t][x] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  for (int64_t b = b0 + wid; b < b1; b += WAVES) {
-    const uint8_t* kb = kp + b * (BT * HD * S1) + lane * 16;
-    const uint8_t* vb = vp + b * (BT * HD * S1) + (F8 ? c * 64 + g * 16 : c * 64 + g * 16);
+  int64_t b = b0 + wid;
+  if (b < b1) {
+    load_k(b);
+    load_v(b);
+  }
+  __builtin_amdgcn_sched_barrier(0);
+  // ---- q into LDS, as a high and a low bf16 part
+  for (int i = tid; i < R * (HD / 8); i += 64 * WAVES) {
+    const int q = i / (HD / 8), d = 8 * (i % (HD / 8));
+    f32x4 v[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    if (rown[q] >= 0) {
+      const f32x4* p = reinterpret_cast<const f32x4*>(&wk.q[((int64_t)rown[q] * A.nh + rowh[q]) * HD + d]);
+      v[0] = p[0], v[1] = p[1];
+    }
+    u32x4 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float a = v[e / 2][2 * (e % 2)], b2 = v[e / 2][2 * (e % 2) + 1];
+      hi[e] = high2(a, b2);
+      lo[e] = f2bf2(copysignf(low<F8>(fabsf(a)), a), copysignf(low<F8>(fabsf(b2)), b2));
+    }
+    *reinterpret_cast<u32x4*>(&qs[0][q * LQ + d]) = hi;
+    *reinterpret_cast<u32x4*>(&qs[1][q * LQ + d]) = lo;
+  }
+  lds_barrier();
+  for (; b < b1; b += WAVES) {
+    asm volatile("" ::: "memory");  // q is read again for each block: held in registers it would push others out
+    // ---- scores
     f32x4 D[RT][4];
 #pragma unroll
     for (int t = 0; t < RT; ++t)
 #pragma unroll
       for (int i = 0; i < 4; ++i) D[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    u32x4 kx, vx;
-    if constexpr (F8) {
-      kx = *reinterpret_cast<const u32x4*>(side.ke + hrow + b * BT + 16 * g);
-      vx = *reinterpret_cast<const u32x4*>(side.ve + hrow + b * BT + 16 * g);
-    }
-    // ---- scores
+    u32x4 q[2][RT][2];  // of this step and the next
+    auto load_q = [&](int s) {
+      const int d = F8 ? 16 * (4 * (s / 2) + g) + 8 * (s % 2) : 8 * (4 * s + g);
 #pragma unroll
-    for (int s = 0; s < KS / (F8 ? 2 : 1); ++s) {
-      u32x4 kr[4];
+      for (int t = 0; t < RT; ++t)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) kr[i] = *reinterpret_cast<const u32x4*>(kb + (s * 4 + i) * 1024);
+        for (int h = 0; h < 2; ++h) q[s % 2][t][h] = *reinterpret_cast<const u32x4*>(&qs[h][(16 * t + c) * LQ + d]);
+    };
+    load_q(0);
 #pragma unroll
-      for (int h = 0; h < (F8 ? 2 : 1); ++h) {
-        u32x4 q[RT];
+    for (int s = 0; s < KS; ++s) {
+      if (s + 1 < KS) load_q(s + 1);
 #pragma unroll
-        for (int t = 0; t < RT; ++t)
-          q[t] = *reinterpret_cast<const u32x4*>(&qs[(16 * t + c) * LQ + (F8 ? 16 * (4 * s + g) + 8 * h : 8 * (4 * s + g))]);
+      for (int i = 0; i < 4; ++i) {
+        const u32x4& k = kr[F8 ? s / 2 * 4 + i : s * 4 + i];
+        const u32x4 a = F8 ? widen(k[s % 2 * 2], k[s % 2 * 2 + 1]) : k;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const u32x4 a = F8 ? widen(kr[i][2 * h], kr[i][2 * h + 1]) : kr[i];
-#pragma unroll
-          for (int t = 0; t < RT; ++t) D[t][i] = mma(a, q[t], D[t][i]);
+        for (int t = 0; t < RT; ++t) {
+          D[t][i] = mma(a, q[s % 2][t][1], D[t][i]);
+          D[t][i] = mma(a, q[s % 2][t][0], D[t][i]);
         }
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
+    const u32x4 kx1 = kx;
+    __builtin_amdgcn_sched_barrier(0);
+    if (b + WAVES < b1) load_k(b + WAVES);
+    else drop(kr);
+    __builtin_amdgcn_sched_barrier(0);
     const int left = (int)(tokens - b * BT < BT ? tokens - b * BT : BT);  // tokens of this block in range
     // ---- softmax of row c over the lane's 16 tokens and the other g's
-    u32x4 pr[RT][2];
+    u32x4 pr[RT][2][2];  // [high and low part][step]
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
       float mx = m[t];
@@ -326,7 +388,7 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void cached_split_kernel(cach
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           float f = scale2;
-          if constexpr (F8) f *= __uint_as_float((kx[i] >> (8 * r) & 0xffu) << 23);
+          if constexpr (F8) f *= __uint_as_float((kx1[i] >> (8 * r) & 0xffu) << 23);
           D[t][i][r] = 16 * g + 4 * i + r < left ? D[t][i][r] * f : -INFINITY;
           mx = fmaxf(mx, D[t][i][r]);
         }
@@ -342,43 +404,45 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void cached_split_kernel(cach
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int r = 0; r < 4; r += 2) {
-          const float p0 = __builtin_amdgcn_exp2f(D[t][i][r] - m0), p1 = __builtin_amdgcn_exp2f(D[t][i][r + 1] - m0);
-          const uint32_t e2 = f2bf2(p0, p1);
-          l[t] += __uint_as_float(e2 << 16) + __uint_as_float(e2 & 0xffff0000u);
-          uint32_t w = e2;
-          if constexpr (F8) {  // a power of two: exact
-            const bool in0 = 16 * g + 4 * i + r < left, in1 = 16 * g + 4 * i + r + 1 < left;
-            const float s0 = __uint_as_float((vx[i] >> (8 * r) & 0xffu) << 23);
-            const float s1 = __uint_as_float((vx[i] >> (8 * r + 8) & 0xffu) << 23);
-            w = f2bf2(in0 ? __uint_as_float(e2 << 16) * s0 : 0.f, in1 ? __uint_as_float(e2 & 0xffff0000u) * s1 : 0.f);
+          float p0 = __builtin_amdgcn_exp2f(D[t][i][r] - m0), p1 = __builtin_amdgcn_exp2f(D[t][i][r + 1] - m0);
+          l[t] += p0 + p1;
+          if constexpr (F8) {  // V's scales, by a select where nothing is in range: a stray scale may be anything
+            const int t0 = 16 * g + 4 * i + r;
+            p0 = t0 < left ? p0 * __uint_as_float((vx[i] >> (8 * r) & 0xffu) << 23) : 0.f;
+            p1 = t0 + 1 < left ? p1 * __uint_as_float((vx[i] >> (8 * r + 8) & 0xffu) << 23) : 0.f;
           }
-          pr[t][i / 2][2 * (i % 2) + r / 2] = w;
+          pr[t][0][i / 2][2 * (i % 2) + r / 2] = high2(p0, p1);
+          pr[t][1][i / 2][2 * (i % 2) + r / 2] = f2bf2(low<F8>(p0), low<F8>(p1));
         }
     }
     // ---- P V
+    if (left < BT) {  // what lies behind the last token may be anything, and 0 times an infinity is NaN
+#pragma unroll
+      for (int i = 0; i < VL; ++i)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          constexpr int TW = 4 / S1;  // tokens per word
+          const int k = left - (16 * g + 8 * (i % S1) + TW * w);
+          vr[i][w] &= k >= TW ? 0xffffffffu : k <= 0 ? 0u : (1u << (32 / TW * k)) - 1u;
+        }
+    }
 #pragma unroll
     for (int x = 0; x < X; ++x) {
-      u32x4 vr[S1];
-#pragma unroll
-      for (int u = 0; u < S1; ++u) vr[u] = *reinterpret_cast<const u32x4*>(vb + x * 1024 * S1 + u * 1024);
-      if (left < BT) {  // what lies behind the last token may be anything, and 0 times an infinity is NaN
-#pragma unroll
-        for (int u = 0; u < S1; ++u)
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            constexpr int TW = 4 / S1;  // tokens per word
-            const int t0 = 16 * g + 8 * u + TW * w, k = left - t0;
-            const uint32_t mask = k >= TW ? 0xffffffffu : k <= 0 ? 0u : (1u << (32 / TW * k)) - 1u;
-            vr[u][w] &= mask;
-          }
-      }
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const u32x4 a = F8 ? widen(vr[0][2 * u], vr[0][2 * u + 1]) : vr[u * (S1 - 1)];
+        const u32x4 a = F8 ? widen(vr[x][2 * u], vr[x][2 * u + 1]) : vr[x * S1 + u * (S1 - 1)];
 #pragma unroll
-        for (int t = 0; t < RT; ++t) O[t][x] = mma(a, pr[t][u], O[t][x]);
+        for (int t = 0; t < RT; ++t) {
+          O[t][x] = mma(a, pr[t][1][u], O[t][x]);
+          O[t][x] = mma(a, pr[t][0][u], O[t][x]);
+        }
       }
+      if (x % 2) __builtin_amdgcn_sched_barrier(0);  // (or every V is widened before the first product)
     }
+    __builtin_amdgcn_sched_barrier(0);
+    if (b + WAVES < b1) load_v(b + WAVES);
+    else drop(vr);
+    __builtin_amdgcn_sched_barrier(0);
   }
   // ---- the waves' sums: one maximum, then DS dims at a time through LDS
 #pragma unroll
@@ -398,7 +462,7 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void cached_split_kernel(cach
     for (int w = 1; w < WAVES; ++w) M[t] = fmaxf(M[t], sm[w][16 * t + c]);
     fix[t] = M[t] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[t] - M[t]);
   }
-  const int at0 = RT == 1 ? part : A.S + part, all = A.S + A.SP;
+  const int at0 = RT == 1 ? part : A.S.parts + part, all = A.S.parts + A.SP.parts;
   if (wid == 0 && g == 0) {
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
@@ -443,19 +507,19 @@ __global__ __launch_bounds__(256) void cached_combine_kernel(cached::Args A, cac
   __shared__ float sl[GR];
   const int n = blockIdx.x / A.nh, h = blockIdx.x % A.nh, t = threadIdx.x, d4 = t % LN, gr = t / LN;
   const Slot s = slot_of(A, n);
-  const int ns = ranges(s.own, A.S), np = s.prefix >= 0 ? ranges(prefix_len(A, s.prefix), A.SP) : 0, all = A.S + A.SP;
+  const int ns = ranges(s.own, A.S), np = s.prefix >= 0 ? ranges(prefix_len(A, s.prefix), A.SP) : 0, all = A.S.parts + A.SP.parts;
   const float* ml = wk.ml + ((int64_t)n * A.nh + h) * all * 2;
   const float* op = wk.o + ((int64_t)n * A.nh + h) * all * HD + 4 * d4;
   const float gate = t < HD ? A.proj(n, (int64_t)h * 2 * HD + HD + t) : 0.f;
   float M = -INFINITY;
-  for (int i = t & 63; i < ns + np; i += 64) M = fmaxf(M, ml[2 * (i < ns ? i : A.S + i - ns)]);
+  for (int i = t & 63; i < ns + np; i += 64) M = fmaxf(M, ml[2 * (i < ns ? i : A.S.parts + i - ns)]);
   M = wave_max_fast(M);
   const float m0 = M == -INFINITY ? 0.f : M;
   float L = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
   for (int i = gr; i < ns + np; i += GR) {
-    const int at = i < ns ? i : A.S + i - ns;
+    const int at = i < ns ? i : A.S.parts + i - ns;
     const float f = __builtin_amdgcn_exp2f(ml[2 * at] - m0);
     L += ml[2 * at + 1] * f;
     o += *reinterpret_cast<const f32x4*>(op + (int64_t)at * HD) * f;
@@ -480,10 +544,10 @@ static int launch_cached(const cached::Args& A, const cached::Work& wk, hipStrea
   const int64_t waves = (int64_t)A.N * (A.nh + 2 * A.nkv);
   const float scale2 = 1.4426950408889634f / sqrtf((float)HD);  // scores in powers of two
   cached_prep_kernel<HD, F8><<<(unsigned)((waves + 3) / 4 + (A.pof ? 1 : 0)), 256, 0, st>>>(A, wk);
-  cached_split_kernel<HD, F8, 1><<<dim3(A.S, A.nkv, A.N), 256, 0, st>>>(A, wk, scale2);
+  cached_split_kernel<HD, F8, 1><<<dim3(A.S.parts, A.nkv, A.N), 256, 0, st>>>(A, wk, scale2);
   if (A.pof)
     cached_split_kernel<HD, F8, 2>
-        <<<dim3(A.SP, A.nkv, A.tiles), 256, 0, st>>>(A, wk, scale2);
+        <<<dim3(A.SP.parts, A.nkv, A.tiles), 256, 0, st>>>(A, wk, scale2);
   cached_combine_kernel<HD><<<A.N * A.nh, 256, 0, st>>>(A, wk);
   return check_launch("gdn_attn_cached");
 }
@@ -494,9 +558,9 @@ using namespace gdn;
 
 namespace {
 // Partials per head of the own tokens and of the prefix.
-void cached_parts(int N, int nh, int nkv, int64_t T, int P, int64_t Tp, int& S, int& SP) {
-  S = cached::parts_of(T, (int64_t)N * nkv);
-  SP = P ? cached::parts_of(Tp, (int64_t)cached::most_tiles(N, nh / nkv, P) * nkv) : 0;
+void cached_cuts(int N, int nh, int nkv, int64_t T, int P, int64_t Tp, cached::Cut& S, cached::Cut& SP) {
+  S = cached::cut_of(T, (int64_t)N * nkv);
+  SP = P ? cached::cut_of(Tp, (int64_t)cached::most_tiles(N, nh / nkv, P) * nkv) : cached::Cut{0, 1};
 }
 bool cached_sizes(int N, int nh, int nkv, int64_t T, int P, int64_t Tp) {
   return N >= 0 && nh >= 1 && nkv >= 1 && nh % nkv == 0 && nkv <= 65535 && N <= 65535 && P >= 0 && T >= kv::BT &&
@@ -507,10 +571,10 @@ bool cached_sizes(int N, int nh, int nkv, int64_t T, int P, int64_t Tp) {
 
 extern "C" int64_t gdn_attn_cached_workspace_bytes(int N, int nh, int nkv, int hd, int64_t T, int P, int64_t Tp) {
   if (!cached_sizes(N, nh, nkv, T, P, Tp) || hd < 1) return -1;
-  int S, SP;
-  cached_parts(N < 1 ? 1 : N, nh, nkv, T, P, Tp, S, SP);
+  cached::Cut S, SP;
+  cached_cuts(N < 1 ? 1 : N, nh, nkv, T, P, Tp, S, SP);
   cached::Work w;
-  return cached::work_of(w, nullptr, N, nh, nkv, hd, S + SP, P);
+  return cached::work_of(w, nullptr, N, nh, nkv, hd, S.parts + SP.parts, P);
 }
 
 extern "C" int gdn_attn_cached(const void* proj, int64_t proj_stride, const float* part, int splits, const int64_t* pos,
@@ -553,9 +617,9 @@ extern "C" int gdn_attn_cached(const void* proj, int64_t proj_stride, const floa
   A.eps = eps;
   A.out = static_cast<uint16_t*>(out);
   A.out_stride = out_stride;
-  cached_parts(N, nh, nkv, T, P, Tp, A.S, A.SP);
+  cached_cuts(N, nh, nkv, T, P, Tp, A.S, A.SP);
   cached::Work wk;
-  const int64_t need = cached::work_of(wk, static_cast<char*>(work), N, nh, nkv, hd, A.S + A.SP, P);
+  const int64_t need = cached::work_of(wk, static_cast<char*>(work), N, nh, nkv, hd, A.S.parts + A.SP.parts, P);
   GDN_REQUIRE(work_bytes >= need, "%s: workspace too small (%lld bytes needed)", name, (long long)need);
   const hipStream_t st = (hipStream_t)stream;
   switch (hd) {
