@@ -6,8 +6,9 @@
 //   o = sum_t p_t v_t / sum_t p_t, p_t = exp(q . k_t / sqrt(hd)), over the slot's prefix and its own tokens;
 //   out = o sigmoid(gate).
 // Launches:
-//   1. cached_prep_kernel: a wave per (slot, head row).  Norm, rotary (angles in double), q to the workspace, k and
-//      v quantised into the cache.  One more workgroup sorts the slots by prefix into tiles of 32 query rows.
+//   1. cached_prep_kernel: a wave per (slot, head row).  Norm, rotary (angles in double), q to the workspace, k and v
+//      quantised into the cache.  One more wave plans: it sorts the slots by prefix into tiles of 32 query rows, and cuts
+//      every slot's own tokens and every tile's prefix into ranges of like cost, a workgroup each.
 //   2. cached_split_kernel: partial softmax sums of a range of tokens for 16 query rows (the G heads of one slot's kv
 //      head) or 32 (a tile of a prefix's slots).
 //   3. cached_combine_kernel: per (slot, head) the partials merged by their maxima, and the gate.
@@ -55,18 +56,6 @@ template <int N> __device__ __forceinline__ void drop(u32x4 (&x)[N]) {
 constexpr int WAVES = 4;       // per split workgroup; a wave takes every 4th block of the range
 constexpr int PROWS = 32;      // query rows of a prefix tile
 
-// Ranges that a row of up to T tokens is cut into (parts at most), of `least` blocks at least: a block per wave where a
-// workgroup for each such range finds room on the chip at once (one fits a CU), else two, and about 4 workgroups a CU
-// where rows are long.
-struct Cut {
-  int parts, least;
-};
-inline Cut cut_of(int64_t T, int64_t items) {
-  const int64_t n = (T + BT - 1) / BT, four = (n + WAVES - 1) / WAVES;
-  const int least = four * items <= 256 ? WAVES : 2 * WAVES;
-  const int64_t most = (n + least - 1) / least, want = (1024 + items - 1) / items;
-  return Cut{(int)(most < want ? most : want), least};
-}
 struct Side {  // one cache: its tensors and its length (tokens, a multiple of 64)
   uint8_t *k, *v, *ke, *ve;
   int64_t T;
@@ -78,37 +67,71 @@ struct Args {
   const float* inv_freq;
   Side own, pre;
   const int32_t *plen, *pof;  // NULL: no prefixes
-  int N, nh, nkv, rd, P, tiles;
-  Cut S, SP;  // partials per head: of the slot's own tokens, of its prefix
+  int N, nh, nkv, rd, P;
+  int items, tiles, own_parts, pre_parts;  // at most so many of each
   float eps;
   uint16_t* out;
   int64_t out_stride;
 };
-// workspace: q (fp32 [N, nh, hd]) | m, l (fp32 [N, nh, S + SP, 2]) | o (fp32 [N, nh, S + SP, hd]) | order (int32 [N]) |
-// tiles (int32 [tiles, 4]: prefix, its first place in order, first row, rows)
+// The plan.  A workgroup's part of the work; a slot's partials; a tile of a prefix's query rows.
+struct Item {
+  int tile;      // -1: a slot's own tokens
+  int row, j;    // cache row (the slot, or the prefix), kv head
+  int b0, b1;    // blocks (b0 = b1: nothing)
+  int tokens;    // of the row
+  int part;      // where its partials go
+  int pad;
+};
+struct SlotPlan {
+  int first, count;  // its own partials
+  int tile, rank;    // its prefix's first tile (-1: none), and its place among that prefix's slots
+};
+struct TilePlan {
+  int prefix, order, row, rows;  // query rows row .. row + rows - 1 of the prefix's slots, which begin at `order`
+  int first, count;              // its partials
+  int pad[2];
+};
+// workspace: q (fp32 [N, nh, hd]) | partials: m, l (fp32 [parts, 2]) and o (fp32 [parts, hd]), parts = own_parts * nkv * G of
+// slots, then pre_parts * nkv * 32 of tiles | the plan
 struct Work {
   float *q, *ml, *o;
-  int32_t* order;
-  int4* tiles;
+  Item* items;
+  SlotPlan* slots;
+  TilePlan* tiles;
+  int32_t* order;  // the slots, prefix after prefix
 };
+constexpr int WGS = 256;   // workgroups planned for where ranges are short: one a CU
+constexpr int LONG = 12;   // blocks of a range when four are planned for each CU
+constexpr int MAXN = 1024, MAXP = 1024;  // slots and prefixes (the plan is made in LDS)
 inline int most_tiles(int N, int G, int P) {  // a prefix of m slots has ceil(m G / 32) tiles
-  const int64_t rows = (int64_t)N * G;
-  const int64_t t = rows / PROWS + (P < N ? P : N);
-  return (int)t;
+  return P ? (int)((int64_t)N * G / PROWS + (P < N ? P : N)) : 0;
 }
 __host__ __device__ inline int64_t round256(int64_t b) { return (b + 255) / 256 * 256; }
-inline int64_t work_of(Work& w, char* p, int N, int nh, int nkv, int hd, int parts, int P) {
+// The plan's bounds: ranges of like cost are at most WGS / nkv + 1 in all (of slots' own tokens 4 times that, if caches of
+// T and prefixes of Tp tokens can hold so many), and one more for each slot and tile (rounding up).
+inline void bound(Args& A, int G, int64_t T, int64_t Tp) {
+  A.tiles = most_tiles(A.N, G, A.P);
+  const int most = WGS / A.nkv + 1;
+  const bool many = (A.N * (T / BT) + 2 * A.tiles * (Tp / BT)) / most + 1 >= 4 * LONG;
+  A.own_parts = (many ? 4 : 1) * most + A.N;
+  A.pre_parts = A.P ? most + A.tiles : 0;
+  A.items = (A.own_parts + A.pre_parts) * A.nkv;
+}
+inline int64_t work_of(Work& w, char* p, const Args& A, int hd) {
   char* const base = p;
-  w.q = reinterpret_cast<float*>(p);
-  p += round256((int64_t)N * nh * hd * 4);
-  w.ml = reinterpret_cast<float*>(p);
-  p += round256((int64_t)N * nh * parts * 8);
-  w.o = reinterpret_cast<float*>(p);
-  p += round256((int64_t)N * nh * parts * hd * 4);
-  w.order = reinterpret_cast<int32_t*>(p);
-  p += P ? round256((int64_t)N * 4) : 0;
-  w.tiles = reinterpret_cast<int4*>(p);
-  p += P ? round256((int64_t)most_tiles(N, nh / nkv, P) * 16) : 0;
+  auto take = [&p](int64_t bytes) {
+    char* q = p;
+    p += round256(bytes);
+    return q;
+  };
+  const int64_t parts = (int64_t)A.own_parts * A.nh + (int64_t)A.pre_parts * A.nkv * PROWS;
+  w.q = reinterpret_cast<float*>(take((int64_t)A.N * A.nh * hd * 4));
+  w.ml = reinterpret_cast<float*>(take(parts * 8));
+  w.o = reinterpret_cast<float*>(take(parts * hd * 4));
+  w.items = reinterpret_cast<Item*>(take((int64_t)A.items * sizeof(Item)));
+  w.slots = reinterpret_cast<SlotPlan*>(take((int64_t)A.N * sizeof(SlotPlan)));
+  w.tiles = reinterpret_cast<TilePlan*>(take((int64_t)A.tiles * sizeof(TilePlan)));
+  w.order = reinterpret_cast<int32_t*>(take(A.P ? (int64_t)A.N * 4 : 0));
   return p - base;
 }
 // What a slot attends to.
@@ -132,45 +155,141 @@ __device__ __forceinline__ Slot slot_of(const Args& A, int n) {
   s.at = at < A.own.T ? at : -1;
   return s;
 }
-// Blocks per range of n blocks.
-__device__ __forceinline__ int64_t range_blocks(int64_t n, const Cut& c) {
-  const int64_t b = (n + c.parts - 1) / c.parts;
-  return b < c.least ? c.least : b;
+__device__ __forceinline__ int blocks(int64_t tokens) { return (int)((tokens + BT - 1) / BT); }
+struct PlanLds {
+  int tokens[MAXN], prefix[MAXN], first[MAXN + 1];
+  int count[MAXP], tile[MAXP + 1], order[MAXP];  // a prefix's slots, first tile, place in order
+  unsigned long long cost;
+  int own, pre, tiles, wave[4];
+};
+// One workgroup of 256 threads.  Ranges cost the same: a block of a tile, with twice the query rows, counts as two of a
+// slot's own.  Ranges are whole turns of a workgroup's waves.
+__device__ __forceinline__ void make_plan(const Args& A, const Work& wk, PlanLds& s) {
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, G = A.nh / A.nkv;
+  if (tid == 0) s.cost = 0;
+  for (int r = tid; r < A.P; r += 256) s.count[r] = 0;
+  __syncthreads();
+  unsigned long long cost = 0;
+  for (int n = tid; n < A.N; n += 256) {
+    const Slot x = slot_of(A, n);
+    s.tokens[n] = (int)x.own;
+    s.prefix[n] = x.prefix;
+    cost += blocks(x.own);
+    if (x.prefix >= 0) atomicAdd(&s.count[x.prefix], 1);
+  }
+  if (cost) atomicAdd(&s.cost, cost);
+  __syncthreads();
+  if (tid == 0) {
+    int tile = 0, order = 0;
+    unsigned long long c = s.cost;
+    for (int r = 0; r < A.P; ++r) {
+      const int nt = (s.count[r] * G + PROWS - 1) / PROWS;
+      s.tile[r] = tile, s.order[r] = order;
+      tile += nt, order += s.count[r];
+      if (nt) c += 2ull * nt * blocks(prefix_len(A, r));
+    }
+    s.tile[A.P] = tile;
+    // a workgroup a CU; of slots' own tokens, which HBM bounds, 4 that even out where there are many blocks (16 slots of
+    // 16384 to 32768 tokens: 199 us with one, 154 with four; 64 slots behind 16384 shared tokens: 105 us with four, 91)
+    unsigned long long each = (c + WGS / A.nkv) / (WGS / A.nkv + 1);
+    if (each > 1 << 28) each = 1 << 28;
+    s.pre = (int)((each + 2 * WAVES - 1) / (2 * WAVES)) * WAVES;
+    if (each >= 4 * LONG) each = (each + 3) / 4;
+    s.own = (int)((each + WAVES - 1) / WAVES) * WAVES;
+  }
+  __syncthreads();
+  // the slots' ranges: thread t's slots are t * per ..
+  const int per = (A.N + 255) / 256;
+  int mine = 0;
+  for (int n = tid * per; n < (tid + 1) * per && n < A.N; ++n) mine += s.own ? (blocks(s.tokens[n]) + s.own - 1) / s.own : 0;
+  int up = mine;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(up, o, kWave);
+    if (lane >= o) up += y;
+  }
+  if (lane == 63) s.wave[wid] = up;
+  __syncthreads();
+  int at = up - mine;
+  for (int w = 0; w < wid; ++w) at += s.wave[w];
+  for (int n = tid * per; n < (tid + 1) * per && n < A.N; ++n) {
+    s.first[n] = at;
+    at += s.own ? (blocks(s.tokens[n]) + s.own - 1) / s.own : 0;
+  }
+  if (tid == 0) s.first[A.N] = s.wave[0] + s.wave[1] + s.wave[2] + s.wave[3];
+  __syncthreads();
+  for (int n = tid; n < A.N; n += 256) {
+    SlotPlan p{s.first[n], s.first[n + 1] - s.first[n], -1, 0};
+    const int r = s.prefix[n];
+    if (r >= 0) {
+      p.tile = s.tile[r];
+      for (int m = 0; m < n; ++m) p.rank += s.prefix[m] == r;
+      wk.order[s.order[r] + p.rank] = n;
+    }
+    wk.slots[n] = p;
+  }
+  // ---- prefixes first, as they are the longest.  A range's tiles lie 8 workgroups apart: on one XCD, whose L2 then
+  // has the range's keys and values for all of them
+  int item = 0, part = 0;
+  for (int r = 0; r < A.P; ++r) {
+    const int t0 = s.tile[r], nt = s.tile[r + 1] - t0, rows = s.count[r] * G;
+    if (!nt) continue;
+    const int tokens = (int)prefix_len(A, r), n = blocks(tokens), parts = n ? (n + s.pre - 1) / s.pre : 0;
+    for (int t = tid; t < nt; t += 256) {
+      const int left = rows - t * PROWS;
+      wk.tiles[t0 + t] = TilePlan{r, s.order[r], t * PROWS, left < PROWS ? left : PROWS, part + t * parts, parts, {0, 0}};
+    }
+    const int units = parts * A.nkv;
+    for (int i = tid; i < units * nt; i += 256) {
+      const int group = i / (8 * nt), in = i % (8 * nt), left = units - 8 * group, w = left < 8 ? left : 8;
+      const int t = in / w, u = 8 * group + in % w, p = u / A.nkv;
+      const int end = (p + 1) * s.pre;
+      wk.items[item + i] = Item{t0 + t, r, u % A.nkv, p * s.pre, end < n ? end : n, tokens, part + t * parts + p, 0};
+    }
+    item += units * nt;
+    part += parts * nt;
+  }
+  // ---- the slots' own tokens
+  const int own = s.first[A.N] * A.nkv;
+  for (int i = tid; item + i < A.items; i += 256) {
+    Item x{-1, 0, 0, 0, 0, 0, 0, 0};
+    if (i < own) {
+      const int f = i / A.nkv;
+      int lo = 0, hi = A.N - 1;  // the last slot that begins at f or before (an empty one begins where the next does)
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (s.first[mid] <= f) lo = mid;
+        else hi = mid - 1;
+      }
+      const int n = blocks(s.tokens[lo]), p = f - s.first[lo], end = (p + 1) * s.own;
+      x = Item{-1, lo, i % A.nkv, p * s.own, end < n ? end : n, s.tokens[lo], f, 0};
+    }
+    wk.items[item + i] = x;
+  }
 }
-__device__ __forceinline__ int ranges(int64_t tokens, const Cut& c) {
-  const int64_t n = (tokens + BT - 1) / BT;
-  const int64_t b = range_blocks(n, c);
-  return (int)((n + b - 1) / b);
-}
+template <int HD, int RT> struct SplitLds {
+  static constexpr int R = 16 * RT, LQ = HD + 8;  // query rows, and their pitch
+  static constexpr int DS = 64;                   // dims per round of the merge
+  alignas(16) uint16_t qs[2][R * LQ];
+  alignas(16) float so[WAVES][R][DS + 4];
+  float sm[WAVES][R], sl[WAVES][R];
+  int rown[R], rowh[R];  // each row's slot (-1: none) and head
+};
 }  // namespace cached
 
-// Workgroup 0..: a wave per (slot, row), rows: nh query heads, nkv keys, nkv values; lane l holds dims l + 64 e.  The last
-// workgroup (with prefixes): the slots in the order of their prefixes, and the tiles.
+// A wave per (slot, row), rows: nh query heads, nkv keys, nkv values; lane l holds dims l + 64 e.  The last workgroup plans.
 template <int HD, bool F8>
 __global__ __launch_bounds__(256) void cached_prep_kernel(cached::Args A, cached::Work wk) {
   using namespace cached;
   constexpr int E = HD / 64;
-  __shared__ float tmp[4][HD];
+  __shared__ union {
+    float tmp[4][HD];
+    PlanLds plan;
+  } lds;
+  auto& tmp = lds.tmp;
   const int wid = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  if (A.pof && blockIdx.x == gridDim.x - 1) {
-    if (wid) return;
-    const int G = A.nh / A.nkv;
-    int at = 0, tile = 0;
-    for (int r = 0; r < A.P; ++r) {
-      const int first = at;
-      for (int n0 = 0; n0 < A.N; n0 += 64) {
-        const int n = n0 + lane;
-        const bool mine = n < A.N && slot_of(A, n).prefix == r;
-        const uint64_t b = __ballot(mine);
-        if (mine) wk.order[at + __popcll(b & ((1ull << lane) - 1))] = n;
-        at += __popcll(b);
-      }
-      const int rows = (at - first) * G;
-      for (int t = 0; t * PROWS < rows; ++t, ++tile)
-        if (lane == 0) wk.tiles[tile] = int4{r, first, t * PROWS, rows - t * PROWS < PROWS ? rows - t * PROWS : PROWS};
-    }
-    for (; tile < A.tiles; ++tile)
-      if (lane == 0) wk.tiles[tile] = int4{0, 0, 0, 0};
+  if (blockIdx.x == gridDim.x - 1) {
+    make_plan(A, wk, lds.plan);
     return;
   }
   const int per = A.nh + 2 * A.nkv;
@@ -236,8 +355,7 @@ __global__ __launch_bounds__(256) void cached_prep_kernel(cached::Args A, cached
   }
 }
 
-// Query rows against a range of tokens.  RT = 1: grid (S, nkv, N), 16 rows, of which G are the slot's heads.  RT = 2: grid
-// (SP, nkv, tiles), 32 rows of a prefix's slots.
+// Query rows against a range of tokens: RT = 1: 16 rows, of which G are the slot's heads; RT = 2: 32 rows of a prefix's slots.
 //
 // Wave w takes blocks w, w + 4, .. of the range; the waves' sums meet in LDS at the end.  Of a block of 64 tokens (lane =
 // (c, g) = (l % 16, l / 16)):
@@ -247,62 +365,54 @@ __global__ __launch_bounds__(256) void cached_prep_kernel(cached::Args A, cached
 //      for token 16 g + 8 u + e: the lane's own scores are its operand.  O's lane (c, g) has row c, dims 16 x + 4 g + r, so
 //      the running maximum's corrections are a number per lane.
 template <int HD, bool F8, int RT>
-__global__ __launch_bounds__(256, RT == 1 && HD < 256 ? 2 : 1) void cached_split_kernel(cached::Args A, cached::Work wk, float scale2) {
+__device__ __forceinline__ void split(const cached::Args& A, const cached::Work& wk, const cached::Item& it, cached::SplitLds<HD, RT>& lds,
+                                      float scale2) {
   using namespace cached;
-  constexpr int R = 16 * RT, LQ = HD + 8;
+  typedef SplitLds<HD, RT> Lds;
+  constexpr int R = Lds::R, LQ = Lds::LQ, DS = Lds::DS;
   constexpr int KS = HD / 32, X = HD / 16;  // 32-dim steps of the scores, 16-dim tiles of the output
-  constexpr int DS = 64;                    // dims per round of the merge
-  __shared__ alignas(16) uint16_t qs[2][R * LQ];
-  __shared__ alignas(16) float so[WAVES][R][DS + 4];
-  __shared__ float sm[WAVES][R], sl[WAVES][R];
-  __shared__ int rown[R], rowh[R];  // each row's slot (-1: none) and head
+  auto& qs = lds.qs;
+  auto& so = lds.so;
+  auto& sm = lds.sm;
+  auto& sl = lds.sl;
+  auto& rown = lds.rown;
+  auto& rowh = lds.rowh;
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int part = blockIdx.x, j = blockIdx.y, G = A.nh / A.nkv;
-  int64_t tokens, row;  // of the cache row
+  const int j = it.j, G = A.nh / A.nkv, tokens = it.tokens;
   const Side& side = RT == 1 ? A.own : A.pre;
-  const Cut& cut = RT == 1 ? A.S : A.SP;
   if (RT == 1) {
-    const int n = blockIdx.z;
-    tokens = slot_of(A, n).own;
-    row = n;
     if (tid < R) {
-      rown[tid] = tid < G ? n : -1;
+      rown[tid] = tid < G ? it.row : -1;
       rowh[tid] = j * G + tid;
     }
   } else {
-    const int4 tile = wk.tiles[blockIdx.z];
-    if (!tile.w) return;  // fewer tiles than there could be
-    tokens = prefix_len(A, tile.x);
-    row = tile.x;
+    const TilePlan tile = wk.tiles[it.tile];
     if (tid < R) {
-      const int q = tile.z + tid;
-      rown[tid] = tid < tile.w ? wk.order[tile.y + q / G] : -1;
+      const int q = tile.row + tid;
+      rown[tid] = tid < tile.rows ? wk.order[tile.order + q / G] : -1;
       rowh[tid] = j * G + q % G;
     }
   }
-  const int64_t nblk = (tokens + BT - 1) / BT, per = range_blocks(nblk, cut);
-  const int64_t b0 = part * per, b1 = b0 + per < nblk ? b0 + per : nblk;
-  if (b0 >= b1) return;
   lds_barrier();
   constexpr int S1 = F8 ? 1 : 2;
   constexpr int KL = HD / 16 * S1, VL = X * S1;  // 16-byte loads of a block's K and V, per lane
   // Loads ahead: the next block's K goes out when this one's scores are done, its V when this one's is used up.
-  const int64_t hrow = (row * A.nkv + j) * side.T;
+  const int64_t hrow = ((int64_t)it.row * A.nkv + j) * side.T;
   const uint8_t* kp = side.k + hrow * HD * S1;
   const uint8_t* vp = side.v + hrow * HD * S1;
   const int kat = lane * 16, vat = c * 64 + g * 16;
   u32x4 kr[KL], vr[VL], kx = {0, 0, 0, 0}, vx = {0, 0, 0, 0};
   // (buffer loads: the block's address is scalar, a lane's offset one register for all of them)
-  auto load_k = [&](int64_t b) {
-    if constexpr (F8) kx = *reinterpret_cast<const u32x4*>(side.ke + hrow + b * BT + 16 * g);
-    const auto block = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(kp) + b * (BT * HD * S1), 0, BT * HD * S1, 0x00027000);
+  auto load_k = [&](int b) {
+    if constexpr (F8) kx = *reinterpret_cast<const u32x4*>(side.ke + hrow + (int64_t)b * BT + 16 * g);
+    const auto block = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(kp) + (int64_t)b * (BT * HD * S1), 0, BT * HD * S1, 0x00027000);
 #pragma unroll
     for (int i = 0; i < KL; ++i) kr[i] = __builtin_amdgcn_raw_buffer_load_b128(block, kat, i * 1024, 0);
   };
-  auto load_v = [&](int64_t b) {
-    if constexpr (F8) vx = *reinterpret_cast<const u32x4*>(side.ve + hrow + b * BT + 16 * g);
-    const auto block = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(vp) + b * (BT * HD * S1), 0, BT * HD * S1, 0x00027000);
+  auto load_v = [&](int b) {
+    if constexpr (F8) vx = *reinterpret_cast<const u32x4*>(side.ve + hrow + (int64_t)b * BT + 16 * g);
+    const auto block = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(vp) + (int64_t)b * (BT * HD * S1), 0, BT * HD * S1, 0x00027000);
 #pragma unroll
     for (int i = 0; i < VL; ++i) vr[i] = __builtin_amdgcn_raw_buffer_load_b128(block, vat, i * 1024, 0);
   };
@@ -315,7 +425,8 @@ __global__ __launch_bounds__(256, RT == 1 && HD < 256 ? 2 : 1) void cached_split
 #pragma unroll
     for (int x = 0; x < X; ++x) O[t][x] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  int64_t b = b0 + wid;
+  const int b1 = it.b1;
+  int b = it.b0 + wid;
   if (b < b1) {
     load_k(b);
     load_v(b);
@@ -377,7 +488,7 @@ __global__ __launch_bounds__(256, RT == 1 && HD < 256 ? 2 : 1) void cached_split
     if (b + WAVES < b1) load_k(b + WAVES);
     else drop(kr);
     __builtin_amdgcn_sched_barrier(0);
-    const int left = (int)(tokens - b * BT < BT ? tokens - b * BT : BT);  // tokens of this block in range
+    const int left = tokens - b * BT < BT ? tokens - b * BT : BT;  // tokens of this block in range
     // ---- softmax of row c over the lane's 16 tokens and the other g's
     u32x4 pr[RT][2][2];  // [high and low part][step]
 #pragma unroll
@@ -462,7 +573,10 @@ __global__ __launch_bounds__(256, RT == 1 && HD < 256 ? 2 : 1) void cached_split
     for (int w = 1; w < WAVES; ++w) M[t] = fmaxf(M[t], sm[w][16 * t + c]);
     fix[t] = M[t] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[t] - M[t]);
   }
-  const int at0 = RT == 1 ? part : A.S.parts + part, all = A.S.parts + A.SP.parts;
+  // partials: G rows of a slot's, or all of a tile's
+  const int NR = RT == 1 ? G : R;
+  const int64_t p0 = RT == 1 ? ((int64_t)it.part * A.nkv + j) * G
+                             : (int64_t)A.own_parts * A.nh + ((int64_t)it.part * A.nkv + j) * R;
   if (wid == 0 && g == 0) {
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
@@ -471,11 +585,7 @@ __global__ __launch_bounds__(256, RT == 1 && HD < 256 ? 2 : 1) void cached_split
 #pragma unroll
       for (int w = 0; w < WAVES; ++w)
         L += M[t] == -INFINITY ? 0.f : sl[w][q] * __builtin_amdgcn_exp2f(sm[w][q] - M[t]);
-      if (rown[q] >= 0) {
-        float* ml = wk.ml + (((int64_t)rown[q] * A.nh + rowh[q]) * all + at0) * 2;
-        ml[0] = M[t];
-        ml[1] = L;
-      }
+      if (rown[q] >= 0) *reinterpret_cast<float2*>(wk.ml + (p0 + q) * 2) = float2{M[t], L};
     }
   }
 #pragma unroll
@@ -486,16 +596,34 @@ __global__ __launch_bounds__(256, RT == 1 && HD < 256 ? 2 : 1) void cached_split
       for (int x = 0; x < DS / 16; ++x)
         *reinterpret_cast<f32x4*>(&so[wid][16 * t + c][16 * x + 4 * g]) = O[t][d0 / 16 + x] * fix[t];
     __syncthreads();
-    for (int i = tid; i < R * (DS / 4); i += 64 * WAVES) {
+    for (int i = tid; i < NR * (DS / 4); i += 64 * WAVES) {
       const int q = i / (DS / 4), d = 4 * (i % (DS / 4));
       f32x4 o = *reinterpret_cast<const f32x4*>(&so[0][q][d]);
 #pragma unroll
       for (int w = 1; w < WAVES; ++w) o += *reinterpret_cast<const f32x4*>(&so[w][q][d]);
       if (rown[q] >= 0)
-        *reinterpret_cast<f32x4*>(&wk.o[(((int64_t)rown[q] * A.nh + rowh[q]) * all + at0) * HD + d0 + d]) = o;
+        *reinterpret_cast<f32x4*>(&wk.o[(p0 + q) * HD + d0 + d]) = o;
     }
     __syncthreads();
   }
+}
+
+// grid (items): a workgroup per item of the plan.  kPre: there may be prefixes.
+template <int HD, bool F8, bool kPre>
+__global__ __launch_bounds__(256, HD < 256 && !kPre ? 2 : 1) void cached_split_kernel(cached::Args A, cached::Work wk, float scale2) {
+  using namespace cached;
+  __shared__ alignas(16) char raw[kPre ? sizeof(SplitLds<HD, 2>) : sizeof(SplitLds<HD, 1>)];
+  Item it = wk.items[blockIdx.x];
+  it.tile = __builtin_amdgcn_readfirstlane(it.tile);
+  it.row = __builtin_amdgcn_readfirstlane(it.row);
+  it.j = __builtin_amdgcn_readfirstlane(it.j);
+  it.b0 = __builtin_amdgcn_readfirstlane(it.b0);
+  it.b1 = __builtin_amdgcn_readfirstlane(it.b1);
+  it.tokens = __builtin_amdgcn_readfirstlane(it.tokens);
+  it.part = __builtin_amdgcn_readfirstlane(it.part);
+  if (it.b0 >= it.b1) return;
+  if (kPre && it.tile >= 0) split<HD, F8, 2>(A, wk, it, *reinterpret_cast<SplitLds<HD, 2>*>(raw), scale2);
+  else split<HD, F8, 1>(A, wk, it, *reinterpret_cast<SplitLds<HD, 1>*>(raw), scale2);
 }
 
 // grid (N * nh), 256 threads: HD / 4 lanes of 4 dims times groups of partials; the groups meet in LDS.
@@ -506,23 +634,35 @@ __global__ __launch_bounds__(256) void cached_combine_kernel(cached::Args A, cac
   __shared__ alignas(16) float so[GR][HD];
   __shared__ float sl[GR];
   const int n = blockIdx.x / A.nh, h = blockIdx.x % A.nh, t = threadIdx.x, d4 = t % LN, gr = t / LN;
-  const Slot s = slot_of(A, n);
-  const int ns = ranges(s.own, A.S), np = s.prefix >= 0 ? ranges(prefix_len(A, s.prefix), A.SP) : 0, all = A.S.parts + A.SP.parts;
-  const float* ml = wk.ml + ((int64_t)n * A.nh + h) * all * 2;
-  const float* op = wk.o + ((int64_t)n * A.nh + h) * all * HD + 4 * d4;
+  const int G = A.nh / A.nkv, j = h / G, g = h % G;
+  const SlotPlan s = wk.slots[n];
+  const int ns = s.count;
+  int np = 0;
+  // partial i of this head: own ones G * nkv apart, a tile's 32 * nkv
+  int64_t first = 0;
+  if (s.tile >= 0) {
+    const int q = s.rank * G + g;
+    const TilePlan tile = wk.tiles[s.tile + q / PROWS];
+    np = tile.count;
+    first = (int64_t)A.own_parts * A.nh + ((int64_t)tile.first * A.nkv + j) * PROWS + q % PROWS;
+  }
+  auto at = [&](int i) {
+    return i < ns ? ((int64_t)(s.first + i) * A.nkv + j) * G + g : first + (int64_t)(i - ns) * A.nkv * PROWS;
+  };
   const float gate = t < HD ? A.proj(n, (int64_t)h * 2 * HD + HD + t) : 0.f;
   float M = -INFINITY;
-  for (int i = t & 63; i < ns + np; i += 64) M = fmaxf(M, ml[2 * (i < ns ? i : A.S.parts + i - ns)]);
+  for (int i = t & 63; i < ns + np; i += 64) M = fmaxf(M, wk.ml[2 * at(i)]);
   M = wave_max_fast(M);
   const float m0 = M == -INFINITY ? 0.f : M;
   float L = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
   for (int i = gr; i < ns + np; i += GR) {
-    const int at = i < ns ? i : A.S.parts + i - ns;
-    const float f = __builtin_amdgcn_exp2f(ml[2 * at] - m0);
-    L += ml[2 * at + 1] * f;
-    o += *reinterpret_cast<const f32x4*>(op + (int64_t)at * HD) * f;
+    const int64_t p = at(i);
+    const float2 ml = *reinterpret_cast<const float2*>(wk.ml + 2 * p);
+    const float f = __builtin_amdgcn_exp2f(ml.x - m0);
+    L += ml.y * f;
+    o += *reinterpret_cast<const f32x4*>(wk.o + p * HD + 4 * d4) * f;
   }
   *reinterpret_cast<f32x4*>(&so[gr][4 * d4]) = o;
   if (d4 == 0) sl[gr] = L;
@@ -543,11 +683,9 @@ template <int HD, bool F8>
 static int launch_cached(const cached::Args& A, const cached::Work& wk, hipStream_t st) {
   const int64_t waves = (int64_t)A.N * (A.nh + 2 * A.nkv);
   const float scale2 = 1.4426950408889634f / sqrtf((float)HD);  // scores in powers of two
-  cached_prep_kernel<HD, F8><<<(unsigned)((waves + 3) / 4 + (A.pof ? 1 : 0)), 256, 0, st>>>(A, wk);
-  cached_split_kernel<HD, F8, 1><<<dim3(A.S.parts, A.nkv, A.N), 256, 0, st>>>(A, wk, scale2);
-  if (A.pof)
-    cached_split_kernel<HD, F8, 2>
-        <<<dim3(A.SP.parts, A.nkv, A.tiles), 256, 0, st>>>(A, wk, scale2);
+  cached_prep_kernel<HD, F8><<<(unsigned)((waves + 3) / 4 + 1), 256, 0, st>>>(A, wk);
+  if (A.pof) cached_split_kernel<HD, F8, true><<<A.items, 256, 0, st>>>(A, wk, scale2);
+  else cached_split_kernel<HD, F8, false><<<A.items, 256, 0, st>>>(A, wk, scale2);
   cached_combine_kernel<HD><<<A.N * A.nh, 256, 0, st>>>(A, wk);
   return check_launch("gdn_attn_cached");
 }
@@ -557,24 +695,20 @@ static int launch_cached(const cached::Args& A, const cached::Work& wk, hipStrea
 using namespace gdn;
 
 namespace {
-// Partials per head of the own tokens and of the prefix.
-void cached_cuts(int N, int nh, int nkv, int64_t T, int P, int64_t Tp, cached::Cut& S, cached::Cut& SP) {
-  S = cached::cut_of(T, (int64_t)N * nkv);
-  SP = P ? cached::cut_of(Tp, (int64_t)cached::most_tiles(N, nh / nkv, P) * nkv) : cached::Cut{0, 1};
-}
 bool cached_sizes(int N, int nh, int nkv, int64_t T, int P, int64_t Tp) {
-  return N >= 0 && nh >= 1 && nkv >= 1 && nh % nkv == 0 && nkv <= 65535 && N <= 65535 && P >= 0 && T >= kv::BT &&
+  return N >= 0 && nh >= 1 && nkv >= 1 && nh % nkv == 0 && nkv <= 65535 && N <= cached::MAXN && P >= 0 && T >= kv::BT &&
          T % kv::BT == 0 && T <= INT32_MAX && (P == 0 || (Tp >= kv::BT && Tp % kv::BT == 0 && Tp <= INT32_MAX)) &&
-         (int64_t)N * nh <= INT32_MAX && P <= 65535;
+         (int64_t)N * nh <= INT32_MAX / 16 && P <= cached::MAXP;
 }
 }  // namespace
 
 extern "C" int64_t gdn_attn_cached_workspace_bytes(int N, int nh, int nkv, int hd, int64_t T, int P, int64_t Tp) {
   if (!cached_sizes(N, nh, nkv, T, P, Tp) || hd < 1) return -1;
-  cached::Cut S, SP;
-  cached_cuts(N < 1 ? 1 : N, nh, nkv, T, P, Tp, S, SP);
+  cached::Args A{};
+  A.N = N, A.nh = nh, A.nkv = nkv, A.P = P;
+  cached::bound(A, nh / nkv, T, P ? Tp : 0);
   cached::Work w;
-  return cached::work_of(w, nullptr, N, nh, nkv, hd, S.parts + SP.parts, P);
+  return cached::work_of(w, nullptr, A, hd);
 }
 
 extern "C" int gdn_attn_cached(const void* proj, int64_t proj_stride, const float* part, int splits, const int64_t* pos,
@@ -586,7 +720,7 @@ extern "C" int gdn_attn_cached(const void* proj, int64_t proj_stride, const floa
                                float eps, void* stream) {
   clear_error();
   const char* name = "gdn_attn_cached";
-  GDN_REQUIRE(cached_sizes(N, nh, nkv, T, P, Tp), "%s: bad head counts, sizes, or a cache length that is no positive multiple of 64", name);
+  GDN_REQUIRE(cached_sizes(N, nh, nkv, T, P, Tp), "%s: bad head counts, more than 1024 slots or prefixes, or a cache length that is no positive multiple of 64", name);
   GDN_REQUIRE(cache_dtype == GDN_BF16 || cache_dtype == GDN_F8E4M3, "%s: the cache's dtype must be bf16 or e4m3", name);
   GDN_SUPPORT(hd == 64 || hd == 128 || hd == 256, "%s: head_dim must be 64, 128 or 256", name);
   GDN_SUPPORT(nh / nkv <= 16, "%s: at most 16 query heads per kv head", name);
@@ -613,13 +747,13 @@ extern "C" int gdn_attn_cached(const void* proj, int64_t proj_stride, const floa
            const_cast<uint8_t*>(pre_k_exp), const_cast<uint8_t*>(pre_v_exp), Tp};
   A.plen = P ? prefix_len : nullptr;
   A.pof = P ? prefix_of : nullptr;
-  A.N = N, A.nh = nh, A.nkv = nkv, A.rd = rd, A.P = P, A.tiles = P ? cached::most_tiles(N, nh / nkv, P) : 0;
+  A.N = N, A.nh = nh, A.nkv = nkv, A.rd = rd, A.P = P;
   A.eps = eps;
   A.out = static_cast<uint16_t*>(out);
   A.out_stride = out_stride;
-  cached_cuts(N, nh, nkv, T, P, Tp, A.S, A.SP);
+  cached::bound(A, nh / nkv, T, P ? Tp : 0);
   cached::Work wk;
-  const int64_t need = cached::work_of(wk, static_cast<char*>(work), N, nh, nkv, hd, A.S.parts + A.SP.parts, P);
+  const int64_t need = cached::work_of(wk, static_cast<char*>(work), A, hd);
   GDN_REQUIRE(work_bytes >= need, "%s: workspace too small (%lld bytes needed)", name, (long long)need);
   const hipStream_t st = (hipStream_t)stream;
   switch (hd) {
