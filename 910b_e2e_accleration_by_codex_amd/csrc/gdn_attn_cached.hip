@@ -261,8 +261,9 @@ __device__ __forceinline__ void make_plan(const Args& A, const Work& wk, PlanLds
         if (s.first[mid] <= f) lo = mid;
         else hi = mid - 1;
       }
-      const int n = blocks(s.tokens[lo]), p = f - s.first[lo], end = (p + 1) * s.own;
-      x = Item{-1, lo, i % A.nkv, p * s.own, end < n ? end : n, s.tokens[lo], f, 0};
+      const int n = blocks(s.tokens[lo]), np = s.first[lo + 1] - s.first[lo], in = i - s.first[lo] * A.nkv;
+      const int p = in % np, end = (p + 1) * s.own;
+      x = Item{-1, lo, in / np, p * s.own, end < n ? end : n, s.tokens[lo], s.first[lo] + p, 0};
     }
     wk.items[item + i] = x;
   }
@@ -459,29 +460,31 @@ __device__ __forceinline__ void split(const cached::Args& A, const cached::Work&
     for (int t = 0; t < RT; ++t)
 #pragma unroll
       for (int i = 0; i < 4; ++i) D[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    u32x4 q[2][RT][2];  // of this step and the next
-    auto load_q = [&](int s) {
+    // (the barriers keep the scheduler from widening every K and reading every q ahead: 256 registers are 2 waves a SIMD)
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      u32x4 q[RT][2];
       const int d = F8 ? 16 * (4 * (s / 2) + g) + 8 * (s % 2) : 8 * (4 * s + g);
 #pragma unroll
       for (int t = 0; t < RT; ++t)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) q[s % 2][t][h] = *reinterpret_cast<const u32x4*>(&qs[h][(16 * t + c) * LQ + d]);
-    };
-    load_q(0);
+        for (int h = 0; h < 2; ++h) q[t][h] = *reinterpret_cast<const u32x4*>(&qs[h][(16 * t + c) * LQ + d]);
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      if (s + 1 < KS) load_q(s + 1);
+      for (int i0 = 0; i0 < 4; i0 += 2) {
+        u32x4 a[2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const u32x4& k = kr[F8 ? s / 2 * 4 + i : s * 4 + i];
-        const u32x4 a = F8 ? widen(k[s % 2 * 2], k[s % 2 * 2 + 1]) : k;
-#pragma unroll
-        for (int t = 0; t < RT; ++t) {
-          D[t][i] = mma(a, q[s % 2][t][1], D[t][i]);
-          D[t][i] = mma(a, q[s % 2][t][0], D[t][i]);
+        for (int i = 0; i < 2; ++i) {
+          const u32x4& k = kr[F8 ? s / 2 * 4 + i0 + i : s * 4 + i0 + i];
+          a[i] = F8 ? widen(k[s % 2 * 2], k[s % 2 * 2 + 1]) : k;
         }
+#pragma unroll
+        for (int h = 1; h >= 0; --h)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int t = 0; t < RT; ++t) D[t][i0 + i] = mma(a[i], q[t][h], D[t][i0 + i]);
+        __builtin_amdgcn_sched_barrier(0);
       }
-      __builtin_amdgcn_sched_barrier(0);
     }
     const u32x4 kx1 = kx;
     __builtin_amdgcn_sched_barrier(0);
@@ -490,6 +493,29 @@ __device__ __forceinline__ void split(const cached::Args& A, const cached::Work&
     __builtin_amdgcn_sched_barrier(0);
     const int left = tokens - b * BT < BT ? tokens - b * BT : BT;  // tokens of this block in range
     // ---- softmax of row c over the lane's 16 tokens and the other g's
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          D[t][i][r] *= F8 ? scale2 * __uint_as_float((kx1[i] >> (8 * r) & 0xffu) << 23) : scale2;
+    if (left < BT) {  // the last block: what lies behind the last token may be anything, and 0 times an infinity is NaN
+      int k = left - 16 * g;  // this lane's tokens in range
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+#pragma unroll
+        for (int t = 0; t < RT; ++t) D[t][i / 4][i % 4] = i < k ? D[t][i / 4][i % 4] : -INFINITY;
+#pragma unroll
+      for (int w = 0; w < 4 * S1; ++w) {  // words of 4 / S1 tokens
+        constexpr int TW = 4 / S1;
+        const int n = k - TW * w;
+        const uint32_t mask = n >= TW ? 0xffffffffu : n <= 0 ? 0u : (1u << (32 / TW * n)) - 1u;
+        if (F8) vx[w % 4] &= mask;
+#pragma unroll
+        for (int x = 0; x < X; ++x) vr[x * S1 + w / 4][w % 4] &= mask;
+      }
+    }
     u32x4 pr[RT][2][2];  // [high and low part][step]
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
@@ -497,12 +523,7 @@ __device__ __forceinline__ void split(const cached::Args& A, const cached::Work&
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float f = scale2;
-          if constexpr (F8) f *= __uint_as_float((kx1[i] >> (8 * r) & 0xffu) << 23);
-          D[t][i][r] = 16 * g + 4 * i + r < left ? D[t][i][r] * f : -INFINITY;
-          mx = fmaxf(mx, D[t][i][r]);
-        }
+        for (int r = 0; r < 4; ++r) mx = fmaxf(mx, D[t][i][r]);
       mx = fmaxf(mx, __shfl_xor(mx, 16, kWave));
       mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
       const float m0 = mx == -INFINITY ? 0.f : mx;
@@ -517,26 +538,15 @@ __device__ __forceinline__ void split(const cached::Args& A, const cached::Work&
         for (int r = 0; r < 4; r += 2) {
           float p0 = __builtin_amdgcn_exp2f(D[t][i][r] - m0), p1 = __builtin_amdgcn_exp2f(D[t][i][r + 1] - m0);
           l[t] += p0 + p1;
-          if constexpr (F8) {  // V's scales, by a select where nothing is in range: a stray scale may be anything
-            const int t0 = 16 * g + 4 * i + r;
-            p0 = t0 < left ? p0 * __uint_as_float((vx[i] >> (8 * r) & 0xffu) << 23) : 0.f;
-            p1 = t0 + 1 < left ? p1 * __uint_as_float((vx[i] >> (8 * r + 8) & 0xffu) << 23) : 0.f;
+          if constexpr (F8) {  // V's scales
+            p0 *= __uint_as_float((vx[i] >> (8 * r) & 0xffu) << 23);
+            p1 *= __uint_as_float((vx[i] >> (8 * r + 8) & 0xffu) << 23);
           }
           pr[t][0][i / 2][2 * (i % 2) + r / 2] = high2(p0, p1);
           pr[t][1][i / 2][2 * (i % 2) + r / 2] = f2bf2(low<F8>(p0), low<F8>(p1));
         }
     }
     // ---- P V
-    if (left < BT) {  // what lies behind the last token may be anything, and 0 times an infinity is NaN
-#pragma unroll
-      for (int i = 0; i < VL; ++i)
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          constexpr int TW = 4 / S1;  // tokens per word
-          const int k = left - (16 * g + 8 * (i % S1) + TW * w);
-          vr[i][w] &= k >= TW ? 0xffffffffu : k <= 0 ? 0u : (1u << (32 / TW * k)) - 1u;
-        }
-    }
 #pragma unroll
     for (int x = 0; x < X; ++x) {
 #pragma unroll
@@ -610,7 +620,7 @@ __device__ __forceinline__ void split(const cached::Args& A, const cached::Work&
 
 // grid (items): a workgroup per item of the plan.  kPre: there may be prefixes.
 template <int HD, bool F8, bool kPre>
-__global__ __launch_bounds__(256, HD < 256 && !kPre ? 2 : 1) void cached_split_kernel(cached::Args A, cached::Work wk, float scale2) {
+__global__ __launch_bounds__(256, !kPre && (HD < 256 || F8) ? 2 : 1) void cached_split_kernel(cached::Args A, cached::Work wk, float scale2) {
   using namespace cached;
   __shared__ alignas(16) char raw[kPre ? sizeof(SplitLds<HD, 2>) : sizeof(SplitLds<HD, 1>)];
   Item it = wk.items[blockIdx.x];
