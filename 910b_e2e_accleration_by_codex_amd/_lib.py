@@ -125,12 +125,13 @@ def call(name, *args):
 
 def call_on(t, name, *args):
     """``call`` with t's device as the current one (a launch goes to the current device's streams only)."""
-    if t.get_device() == torch.cuda.current_device():
+    if t.get_device() == _current_device():
         return call(name, *args)
     with torch.cuda.device(t.device):
         return call(name, *args)
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 

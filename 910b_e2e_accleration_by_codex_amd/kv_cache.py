@@ -18,6 +18,7 @@ from .gdn_chunk_fast import Rows, Varlen, _to_device_int32
 
 F8 = torch.float8_e4m3fn
 _BLOCK = 64
+_NO_PREFIX = (None,) * 6
 
 
 class KVCache(NamedTuple):
@@ -61,31 +62,33 @@ class SharedPrefix(NamedTuple):
     of: torch.Tensor
 
 
+# (these run once per layer and step: each attribute of a tensor that Python looks at costs a good part of a microsecond)
 def _check(name, c):
-    """(cache dtype code, rows, kv heads, head_dim, length) of a well-formed cache."""
+    """(cache dtype code, rows, kv heads, head_dim, length, device index) of a well-formed cache."""
     k, v, ke, ve = c
-    _lib.require_cuda(k, v, ke, ve)
-    if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or not (k.is_contiguous() and v.is_contiguous()):
-        raise ValueError(f"{name}: a cache's k and v are contiguous tensors [R, kv, T / 64, 64 * hd] of one dtype")
-    R, kv, blocks, width = k.shape
-    if width % _BLOCK or width // _BLOCK not in (64, 128, 256) or blocks < 1:
-        raise ValueError(f"{name}: head_dim must be 64, 128 or 256 (got {tuple(k.shape)} = [R, kv, T / 64, 64 * hd])")
-    if k.dtype == F8:
-        want = (R, kv, blocks * _BLOCK)
-        if ke is None or ve is None or ke.shape != want or ve.shape != want or ke.dtype != torch.uint8 \
-                or ve.dtype != torch.uint8 or not (ke.is_contiguous() and ve.is_contiguous()):
-            raise ValueError(f"{name}: an e4m3 cache needs contiguous uint8 k_exp and v_exp {list(want)}")
-        code = _lib.F8E4M3
-    elif k.dtype == torch.bfloat16:
-        if ke is not None or ve is not None:
-            raise ValueError(f"{name}: a bf16 cache has no scales")
-        code = _lib.BF16
-    else:
-        raise TypeError(f"{name}: a cache is bfloat16 or float8_e4m3fn, got {k.dtype}")
-    if k.get_device() != v.get_device() or (ke is not None and (ke.get_device() != k.get_device()
-                                                               or ve.get_device() != k.get_device())):
+    shape, dtype, dev = k.shape, k.dtype, k.get_device()
+    if dev < 0 or v.get_device() != dev:
+        _lib.require_cuda(k, v, ke, ve)
         raise ValueError(f"{name}: a cache's tensors must be on one device")
-    return code, R, kv, width // _BLOCK, blocks * _BLOCK
+    if len(shape) != 4 or shape != v.shape or dtype is not v.dtype or not (k.is_contiguous() and v.is_contiguous()):
+        raise ValueError(f"{name}: a cache's k and v are contiguous tensors [R, kv, T / 64, 64 * hd] of one dtype")
+    R, kv, blocks, width = shape
+    if width not in (4096, 8192, 16384) or blocks < 1:
+        raise ValueError(f"{name}: head_dim must be 64, 128 or 256 (got {tuple(shape)} = [R, kv, T / 64, 64 * hd])")
+    T = blocks * _BLOCK
+    if dtype is F8:
+        want = (R, kv, T)
+        if ke is None or ve is None or ke.shape != want or ve.shape != want or ke.dtype is not torch.uint8 \
+                or ve.dtype is not torch.uint8 or not (ke.is_contiguous() and ve.is_contiguous()):
+            raise ValueError(f"{name}: an e4m3 cache needs contiguous uint8 k_exp and v_exp {list(want)}")
+        if ke.get_device() != dev or ve.get_device() != dev:
+            raise ValueError(f"{name}: a cache's tensors must be on one device")
+        return _lib.F8E4M3, R, kv, width // _BLOCK, T, dev
+    if dtype is not torch.bfloat16:
+        raise TypeError(f"{name}: a cache is bfloat16 or float8_e4m3fn, got {dtype}")
+    if ke is not None or ve is not None:
+        raise ValueError(f"{name}: a bf16 cache has no scales")
+    return _lib.BF16, R, kv, width // _BLOCK, T, dev
 
 
 def _int32(name, what, x, n, device):
@@ -95,9 +98,9 @@ def _int32(name, what, x, n, device):
     if n is not None and x.numel() != n:
         raise ValueError(f"{name}: {what} must have {n} entries, got {x.numel()}")
     if x.is_cuda:
-        if x.dtype != torch.int32 or x.device != device:
+        if x.dtype is not torch.int32 or x.get_device() != device.index:
             raise ValueError(f"{name}: {what} on the device must be int32 on {device}")
-        return x.reshape(-1).contiguous()
+        return x if x.dim() == 1 and x.is_contiguous() else x.reshape(-1).contiguous()
     if x.dtype.is_floating_point or x.dtype == torch.bool:
         raise TypeError(f"{name}: {what} must be whole numbers")
     return _to_device_int32(x.reshape(-1).to(torch.int64), device)
@@ -147,14 +150,14 @@ def kv_cache_store(cache, k, v, rows, cu_seqlens=None, start=None):
     int32 tensors on the device, or lists / CPU tensors (a Rows / Varlen where one is at hand).  Rows and positions outside the
     cache are not written; no two sequences may write the same place."""
     name = "kv_cache_store"
-    code, R, kv, hd, T = _check(name, cache)
+    code, R, kv, hd, T, index = _check(name, cache)
     _lib.require_cuda(k, v)
-    if k.dim() != 3 or k.shape != v.shape or tuple(k.shape[1:]) != (kv, hd) or k.dtype != v.dtype:
+    if k.dim() != 3 or k.shape != v.shape or k.shape[1] != kv or k.shape[2] != hd or k.dtype is not v.dtype:
         raise ValueError(f"{name}: k and v must be [tokens, {kv}, {hd}] of one dtype, got {tuple(k.shape)} {k.dtype} and "
                          f"{tuple(v.shape)} {v.dtype}")
     in_code = _lib.dtype_code(k)
     dev = cache.k.device
-    if k.device != dev or v.device != dev:
+    if k.get_device() != index or v.get_device() != index:
         raise ValueError(f"{name}: k and v must be on the cache's device {dev}")
     total = k.shape[0]
     rows, cu, start, nseq = _batch(name, rows, cu_seqlens, start, total, R, dev)
@@ -175,7 +178,7 @@ def kv_cache_load(cache, rows, cu_seqlens, start=None, total_tokens=None):
     ``total_tokens`` (its last entry) too, or it is read back.  Returns (k, v) [total_tokens, kv, hd] bf16; positions and
     rows outside the cache are zeros."""
     name = "kv_cache_load"
-    code, R, kv, hd, T = _check(name, cache)
+    code, R, kv, hd, T, _ = _check(name, cache)
     dev = cache.k.device
     if total_tokens is None:
         if cu_seqlens is None:
@@ -199,7 +202,7 @@ def cached_attn_workspace(cache, n_heads, prefix=None):
     """The workspace cached_decode_attention needs for this cache and prefix cache (allocate once, reuse per layer and
     step; calls that may overlap need one each)."""
     name = "cached_attn_workspace"
-    _, N, kv, hd, T = _check(name, cache)
+    _, N, kv, hd, T, _ = _check(name, cache)
     P, Tp = (prefix.cache.k.shape[0], prefix.cache.length) if prefix is not None else (0, 0)
     nbytes = int(_lib.lib().gdn_attn_cached_workspace_bytes(N, n_heads, kv, hd, T, P, Tp))
     if nbytes < 0:
@@ -216,46 +219,50 @@ def cached_decode_attention(proj, pos, q_norm, k_norm, inv_freq, cache, n_heads,
     well; pos counts from the prefix's beginning, and the slot's own row holds what follows it.  Returns the gated output
     [N, nh * hd] bf16.  Capturable in a graph (with ``work`` kept by the caller)."""
     name = "cached_decode_attention"
-    code, N, kv, hd, T = _check(name, cache)
-    nh, dev = n_heads, cache.k.device
+    code, N, kv, hd, T, dev = _check(name, cache)
+    nh = n_heads
+    width = (2 * nh + 2 * kv) * hd
     part = proj if isinstance(proj, Partials) else None
     if part is not None:
-        if part.N != (2 * nh + 2 * kv) * hd:
-            raise ValueError(f"{name}: partials of a [(2 nh + 2 kv) hd]-wide projection expected")
         proj = part.data[0]
-    _lib.require_cuda(proj, pos, q_norm, k_norm)
-    if ((proj.dtype != torch.bfloat16 and part is None) or proj.dim() != 2 or tuple(proj.shape) != (N, (2 * nh + 2 * kv) * hd)
-            or pos.dtype != torch.int64 or pos.numel() != N):
-        raise ValueError(f"{name}: bf16 proj [N, (2 nh + 2 kv) hd] and int64 pos [N] for the cache's N = {N} rows expected")
+    elif proj.dtype is not torch.bfloat16:
+        raise ValueError(f"{name}: proj must be bfloat16, got {proj.dtype}")
+    if proj.shape != (N, width) or pos.dtype is not torch.int64 or pos.numel() != N:
+        _lib.require_cuda(proj, pos)
+        raise ValueError(f"{name}: bf16 proj [N, (2 nh + 2 kv) hd] = [{N}, {width}] (or partials of that width) and int64 pos [N] "
+                         f"for the cache's N = {N} rows expected")
     if q_norm.numel() != hd or k_norm.numel() != hd:
         raise ValueError(f"{name}: q_norm and k_norm must have head_dim = {hd} entries")
     if rotary_dim and inv_freq.numel() != rotary_dim // 2:
         raise ValueError(f"{name}: inv_freq must have rotary_dim / 2 = {rotary_dim // 2} entries")
-    if any(t.device != dev for t in (proj, pos, q_norm, k_norm)) or (rotary_dim and inv_freq.device != dev):
-        raise ValueError(f"{name}: every tensor must be on the cache's device {dev}")
+    if proj.get_device() != dev or pos.get_device() != dev or q_norm.get_device() != dev or k_norm.get_device() != dev \
+            or (rotary_dim and inv_freq.get_device() != dev):
+        _lib.require_cuda(proj, pos, q_norm, k_norm)
+        raise ValueError(f"{name}: every tensor must be on the cache's device {cache.k.device}")
     if part is None and proj.stride(1) != 1:
         proj = proj.contiguous()
-    P, Tp, pre = 0, 0, (None,) * 6
+    P, Tp, pre = 0, 0, _NO_PREFIX
     if prefix is not None:
-        pc, P, pkv, phd, Tp = _check(name, prefix.cache)
-        if (pc, pkv, phd) != (code, kv, hd) or prefix.cache.k.device != dev:
+        pc, P, pkv, phd, Tp, pdev = _check(name, prefix.cache)
+        if (pc, pkv, phd, pdev) != (code, kv, hd, dev):
             raise ValueError(f"{name}: the prefix cache must have the cache's dtype, kv heads, head_dim and device")
         for what, x, n in (("length", prefix.length, P), ("of", prefix.of, N)):
-            if not x.is_cuda or x.device != dev or x.dtype != torch.int32 or x.numel() != n or not x.is_contiguous():
-                raise ValueError(f"{name}: prefix.{what} must be a contiguous int32 tensor of {n} entries on {dev}")
+            if x.get_device() != dev or x.dtype is not torch.int32 or x.numel() != n or not x.is_contiguous():
+                raise ValueError(f"{name}: prefix.{what} must be a contiguous int32 tensor of {n} entries on the cache's device")
         c = prefix.cache
         pre = (c.k.data_ptr(), c.v.data_ptr(), _lib.ptr(c.k_exp), _lib.ptr(c.v_exp), prefix.length.data_ptr(),
                prefix.of.data_ptr())
-    qn = q_norm.to(torch.bfloat16).contiguous()
-    kn = k_norm.to(torch.bfloat16).contiguous()
-    inv = inv_freq.to(torch.float32).contiguous() if rotary_dim else None
-    pos = pos.contiguous()
+    qn = q_norm if q_norm.dtype is torch.bfloat16 and q_norm.is_contiguous() else q_norm.to(torch.bfloat16).contiguous()
+    kn = k_norm if k_norm.dtype is torch.bfloat16 and k_norm.is_contiguous() else k_norm.to(torch.bfloat16).contiguous()
+    inv = _lib.f32_dense(inv_freq) if rotary_dim else None
+    if not pos.is_contiguous():
+        pos = pos.contiguous()
     if work is None:
         work = cached_attn_workspace(cache, nh, prefix)
-    elif not work.is_cuda or work.device != dev or not work.is_contiguous():
-        raise ValueError(f"{name}: work must be a contiguous tensor on {dev}")
-    out = torch.empty(N, nh * hd, dtype=torch.bfloat16, device=dev)
-    stride = proj.stride(0) if N > 1 else proj.shape[1]
+    elif work.get_device() != dev or not work.is_contiguous():
+        raise ValueError(f"{name}: work must be a contiguous tensor on the cache's device")
+    out = proj.new_empty((N, nh * hd), dtype=torch.bfloat16)
+    stride = proj.stride(0) if N > 1 else width
     _lib.call_on(proj, "gdn_attn_cached", None if part is not None else proj.data_ptr(), stride,
               None if part is None else part.data.data_ptr(), 0 if part is None else part.splits,
               pos.data_ptr(), qn.data_ptr(), kn.data_ptr(), _lib.ptr(inv), cache.k.data_ptr(),
