@@ -47,6 +47,14 @@ template <bool F8> __device__ __forceinline__ float low(float x) {  // x >= 0
   const float r = x - __uint_as_float(__float_as_uint(x) & 0xffff0000u);
   return F8 ? r : fmaxf(r, x > 0.f ? 0x1p-126f : 0.f);
 }
+// The scheduler is asked for N products, each followed by an arithmetic instruction.
+template <int N> __device__ __forceinline__ void mix() {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x2, 1, 0);
+  }
+}
 // The registers' values are not needed any more: without this, a load that only one branch does keeps the other branch's old
 // values alive.
 template <int N> __device__ __forceinline__ void drop(u32x4 (&x)[N]) {
@@ -460,29 +468,42 @@ __device__ __forceinline__ void split(const cached::Args& A, const cached::Work&
     for (int t = 0; t < RT; ++t)
 #pragma unroll
       for (int i = 0; i < 4; ++i) D[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    // (the barriers keep the scheduler from widening every K and reading every q ahead: 256 registers are 2 waves a SIMD)
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      u32x4 q[RT][2];
+    // Operands of a step: q, and K of its 4 tiles.  With 32 query rows, one wave a SIMD, the next step's e4m3 codes are
+    // widened among this one's products; with 16, two waves a SIMD fill each other's gaps, and 256 registers are all there
+    // are: two tiles at a time (6 registers too many, in scratch: 158 -> 186 us for 16 slots of 16384 to 32768 tokens).
+    constexpr int AHEAD = RT == 2 && F8 ? 1 : 0, W = AHEAD ? 4 : 2;
+    u32x4 a[AHEAD + 1][W], q[AHEAD + 1][RT][2];
+    auto query = [&](int s) {
       const int d = F8 ? 16 * (4 * (s / 2) + g) + 8 * (s % 2) : 8 * (4 * s + g);
 #pragma unroll
       for (int t = 0; t < RT; ++t)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) q[t][h] = *reinterpret_cast<const u32x4*>(&qs[h][(16 * t + c) * LQ + d]);
+        for (int h = 0; h < 2; ++h)
+          q[s % (AHEAD + 1)][t][h] = *reinterpret_cast<const u32x4*>(&qs[h][(16 * t + c) * LQ + d]);
+    };
+    auto keys = [&](int s, int i0) {
 #pragma unroll
-      for (int i0 = 0; i0 < 4; i0 += 2) {
-        u32x4 a[2];
+      for (int i = 0; i < W; ++i) {
+        const u32x4& k = kr[F8 ? s / 2 * 4 + i0 + i : s * 4 + i0 + i];
+        a[s % (AHEAD + 1)][i] = F8 ? widen(k[s % 2 * 2], k[s % 2 * 2 + 1]) : k;
+      }
+    };
+    if (AHEAD) query(0), keys(0, 0);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const u32x4& k = kr[F8 ? s / 2 * 4 + i0 + i : s * 4 + i0 + i];
-          a[i] = F8 ? widen(k[s % 2 * 2], k[s % 2 * 2 + 1]) : k;
-        }
+    for (int s = 0; s < KS; ++s) {
+      if (!AHEAD) query(s);
+      else if (s + 1 < KS) query(s + 1), keys(s + 1, 0);
+#pragma unroll
+      for (int i0 = 0; i0 < 4; i0 += W) {
+        if (!AHEAD) keys(s, i0);
 #pragma unroll
         for (int h = 1; h >= 0; --h)
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
+          for (int i = 0; i < W; ++i)
 #pragma unroll
-            for (int t = 0; t < RT; ++t) D[t][i0 + i] = mma(a[i], q[t][h], D[t][i0 + i]);
+            for (int t = 0; t < RT; ++t)
+              D[t][i0 + i] = mma(a[s % (AHEAD + 1)][i], q[s % (AHEAD + 1)][t][h], D[t][i0 + i]);
+        if (AHEAD) mix<16>();
         __builtin_amdgcn_sched_barrier(0);
       }
     }
@@ -547,18 +568,32 @@ __device__ __forceinline__ void split(const cached::Args& A, const cached::Work&
         }
     }
     // ---- P V
+    constexpr int WV = AHEAD ? 2 : 1;  // 16-dim tiles at a time
+    u32x4 v[2 * AHEAD + 1][WV];
+    auto values = [&](int y, int u) {
 #pragma unroll
-    for (int x = 0; x < X; ++x) {
+      for (int x = 0; x < WV; ++x) {
+        const int at = WV * y + x;
+        v[(2 * y + u) % (2 * AHEAD + 1)][x] = F8 ? widen(vr[at][2 * u], vr[at][2 * u + 1]) : vr[at * S1 + u * (S1 - 1)];
+      }
+    };
+    if (AHEAD) values(0, 0), values(0, 1);
+#pragma unroll
+    for (int y = 0; y < X / WV; ++y) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const u32x4 a = F8 ? widen(vr[x][2 * u], vr[x][2 * u + 1]) : vr[x * S1 + u * (S1 - 1)];
+        if (!AHEAD) values(y, u);
+        else if (y + 1 < X / WV) values(y + 1, u);
 #pragma unroll
-        for (int t = 0; t < RT; ++t) {
-          O[t][x] = mma(a, pr[t][1][u], O[t][x]);
-          O[t][x] = mma(a, pr[t][0][u], O[t][x]);
-        }
+        for (int h = 1; h >= 0; --h)
+#pragma unroll
+          for (int x = 0; x < WV; ++x)
+#pragma unroll
+            for (int t = 0; t < RT; ++t)
+              O[t][WV * y + x] = mma(v[(2 * y + u) % (2 * AHEAD + 1)][x], pr[t][h][u], O[t][WV * y + x]);
       }
-      if (x % 2) __builtin_amdgcn_sched_barrier(0);  // (or every V is widened before the first product)
+      if (AHEAD) mix<16>();
+      if (AHEAD || y % 2) __builtin_amdgcn_sched_barrier(0);  // (or every V is widened before the first product)
     }
     __builtin_amdgcn_sched_barrier(0);
     if (b + WAVES < b1) load_v(b + WAVES);
