@@ -40,6 +40,14 @@ template <> __device__ __forceinline__ void load16(const _Float16* p, float (&x)
   }
 }
 
+// Bytes of 4 words transposed: word i's byte j becomes word j's byte i.
+__device__ __forceinline__ void transpose4(uint32_t (&w)[4]) {
+  const uint32_t a = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u), b = __builtin_amdgcn_perm(w[1], w[0], 0x07030602u);
+  const uint32_t c = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u), d = __builtin_amdgcn_perm(w[3], w[2], 0x07030602u);
+  w[0] = __builtin_amdgcn_perm(c, a, 0x05040100u), w[1] = __builtin_amdgcn_perm(c, a, 0x07060302u);
+  w[2] = __builtin_amdgcn_perm(d, b, 0x05040100u), w[3] = __builtin_amdgcn_perm(d, b, 0x07060302u);
+}
+
 // A batch of sequences: sequence s is the packed tokens [lo, hi), which lie at positions start + 0, 1, .. of cache row
 // `row`.  Nothing here is trusted: token ranges are cut to [0, total), a row outside [0, n_rows) is -1.
 struct Batch {
@@ -157,37 +165,48 @@ __global__ __launch_bounds__(256) void kv_store_kernel(const T* __restrict__ xk,
   }
   if (!is_v) return;
   __syncthreads();
-  // V: 16 bytes (16 / S tokens of one dim) at a time, in the order in which they lie in the cache
-  constexpr int TK = 16 / S;
+  constexpr int TK = 16 / S;  // tokens of 16 bytes of V
+  auto put = [&](uint8_t* at, const uint32_t (&w)[4], int t) {  // tokens t .. t + TK - 1 of one dim
+    const int64_t first = q.lo + (t0 + t - q.start);
+    if (first >= q.lo && first + TK <= q.hi) {
+      *reinterpret_cast<u32x4*>(at) = u32x4{w[0], w[1], w[2], w[3]};
+      return;
+    }
+#pragma unroll
+    for (int e = 0; e < TK; ++e)  // tokens outside the sequence stay as they are
+      if (first + e >= q.lo && first + e < q.hi) {
+        if constexpr (F8) at[e] = (uint8_t)(w[e / 4] >> (8 * (e % 4)));
+        else reinterpret_cast<uint16_t*>(at)[e] = (uint16_t)(w[e / 2] >> (16 * (e % 2)));
+      }
+  };
+  if constexpr (F8) {  // 4 dims of 16 tokens a thread: 16 words from LDS (byte by byte: 64), 4 x 4 bytes transposed in registers
+    for (int o = tid; o < HD; o += 256) {
+      const int a = o % 4, d = o / 4 * 4;
+      uint32_t w[4][4];  // [dim][4 tokens]
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const uint32_t*>(&tile[(16 * a + 4 * j + i) * PITCH + d]);
+        transpose4(x);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i][j] = x[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) put(out + (int64_t)(d + i) * 64 + 16 * a, w[i], 16 * a);
+    }
+    return;
+  }
+  // 16 bytes (8 tokens of one dim) at a time, in the order in which they lie in the cache
   for (int o = tid; o < HD * BT * S / 16; o += 256) {
     const int dg = o / (64 * S), rest = o % (64 * S);  // 16 dims, then [16 dims][4] (e4m3) or [2][16 dims][4] (bf16)
     const int u = rest / 64, m = rest / 4 % 16, a = rest % 4, d = 16 * dg + m, t = 16 * a + 8 * u;
     uint32_t w[4];
-    bool full = true;
-    if constexpr (F8) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        w[j] = tile[(t + 4 * j) * PITCH + d] | tile[(t + 4 * j + 1) * PITCH + d] << 8 |
-               tile[(t + 4 * j + 2) * PITCH + d] << 16 | (uint32_t)tile[(t + 4 * j + 3) * PITCH + d] << 24;
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        w[j] = *reinterpret_cast<const uint16_t*>(&tile[(t + 2 * j) * PITCH + 2 * d]) |
-               (uint32_t) * reinterpret_cast<const uint16_t*>(&tile[(t + 2 * j + 1) * PITCH + 2 * d]) << 16;
-    }
-    const int64_t first = q.lo + (t0 + t - q.start);
-    full = first >= q.lo && first + TK <= q.hi;
-    uint8_t* at = out + (int64_t)o * 16;
-    if (full) {
-      *reinterpret_cast<u32x4*>(at) = u32x4{w[0], w[1], w[2], w[3]};
-    } else {  // tokens outside the sequence stay as they are
-#pragma unroll
-      for (int e = 0; e < TK; ++e)
-        if (first + e >= q.lo && first + e < q.hi) {
-          if constexpr (F8) at[e] = (uint8_t)(w[e / 4] >> (8 * (e % 4)));
-          else reinterpret_cast<uint16_t*>(at)[e] = (uint16_t)(w[e / 2] >> (16 * (e % 2)));
-        }
-    }
+    for (int j = 0; j < 4; ++j)
+      w[j] = *reinterpret_cast<const uint16_t*>(&tile[(t + 2 * j) * PITCH + 2 * d]) |
+             (uint32_t) * reinterpret_cast<const uint16_t*>(&tile[(t + 2 * j + 1) * PITCH + 2 * d]) << 16;
+    put(out + (int64_t)o * 16, w, t);
   }
 }
 
@@ -212,7 +231,21 @@ __global__ __launch_bounds__(256) void kv_load_kernel(const uint8_t* __restrict_
   const bool is_v = blockIdx.z;
   const int64_t row = (int64_t)q.row * nkv + head;
   const uint8_t* in = (is_v ? vc : kc) + (row * len + t0) * HD * S;
-  if (is_v && there) {
+  if (is_v && there && F8) {
+    for (int o = tid; o < HD; o += 256) {
+      const int a = o % 4, d = o / 4 * 4;
+      u32x4 w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const u32x4*>(in + (int64_t)(d + i) * 64 + 16 * a);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t x[4] = {w[0][j], w[1][j], w[2][j], w[3][j]};
+        transpose4(x);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) *reinterpret_cast<uint32_t*>(&tile[(16 * a + 4 * j + i) * PITCH + d]) = x[i];
+      }
+    }
+  } else if (is_v && there) {
     for (int o = tid; o < HD * BT * S / 16; o += 256) {
       const int dg = o / (64 * S), rest = o % (64 * S);
       const int u = rest / 64, m = rest / 4 % 16, a = rest % 4, d = 16 * dg + m, t = 16 * a + 8 * u;
