@@ -13,7 +13,9 @@ gdn_decode_linear), the residual adds with their RMSNorms and the SwiGLU product
 kernels; the output projections hand their split-K partial sums straight to the residual add + norm,
 and gate_up its partials to SwiGLU.  The attention layer (q/k norms, rotary, cache writes, softmax
 attention, gate) is this library's three-launch decode attention.  The KV cache keeps K transposed
-([slot, kv head, head_dim, position]) so the score loads run along positions.
+([slot, kv head, head_dim, position]) so the score loads run along positions.  With ``cache_dtype`` the layers keep
+KVCaches instead (bf16, or e4m3 at half the bytes), and with ``prefix_ctx`` the slots continue one prefix that is stored
+and read once for all of them; ``sample`` draws the step's tokens from its logits.
 """
 from dataclasses import dataclass
 from types import SimpleNamespace
@@ -22,6 +24,8 @@ import torch
 
 from .cb_engine import (GDNSlots, PackedWeight, add_rms_norm, attn_decode_workspace, decode_linear, decode_linear_partial,
                         gdn_decode_core, gqa_decode_attention, swiglu)
+from .kv_cache import KVCache, SharedPrefix, cached_attn_workspace, cached_decode_attention, kv_cache_store
+from .sampling import sample_tokens, sample_workspace
 
 
 @dataclass
@@ -57,9 +61,15 @@ class HybridDecoder:
     """Random-weight hybrid stack with slot state for ``n_slots`` sequences.  ``ctx`` (int [N], host)
     are the per-slot context lengths already in the caches; each ``step`` appends one token per slot.
     Every linear weight is packed once for the decode projection kernel (``L.<name>_p``); the plain
-    [N, K] weights are kept only with ``keep_plain`` (for checks against a reference)."""
+    [N, K] weights are kept only with ``keep_plain`` (for checks against a reference).
+    ``cache_dtype`` (torch.bfloat16 or torch.float8_e4m3fn): the attention layers' histories in KVCaches of that type.
+    ``prefix_ctx`` (with cache_dtype): tokens of a prefix that every slot continues, so that ctx counts what is the slots'
+    own and the next position is prefix_ctx + ctx."""
 
-    def __init__(self, cfg, n_slots, ctx, max_steps, device, seed=0, weight_std=0.02, keep_plain=False):
+    def __init__(self, cfg, n_slots, ctx, max_steps, device, seed=0, weight_std=0.02, keep_plain=False, cache_dtype=None,
+                 prefix_ctx=0):
+        if prefix_ctx and cache_dtype is None:
+            raise ValueError("HybridDecoder: a shared prefix needs a cache_dtype")
         self.cfg, self.N, self.dev = cfg, n_slots, device
         g_ = torch.Generator(device=device).manual_seed(seed)
         bf = torch.bfloat16
@@ -73,7 +83,9 @@ class HybridDecoder:
         self.slots = GDNSlots(n_slots, gdn_ids, cfg.conv_dim, cfg.conv_k, cfg.gdn_v_heads, D, device)
         ctx = torch.as_tensor(ctx, dtype=torch.int64)
         self.max_ctx = (int(ctx.max()) + max_steps + 3) // 4 * 4  # the attention kernels read 4 positions at once
-        self.pos = ctx.to(device=device, dtype=torch.int64)  # position of the next token per slot
+        self.pos = ctx.to(device=device, dtype=torch.int64) + prefix_ctx  # position of the next token per slot
+        self.prefix_len = torch.full((1,), prefix_ctx, dtype=torch.int32, device=device)
+        self.prefix_of = torch.zeros(n_slots, dtype=torch.int32, device=device)
         kv, hd = cfg.kv_heads, cfg.attn_head
         for i in range(cfg.layers):
             L = SimpleNamespace(full=cfg.is_full(i), in_norm=w(H), post_norm=w(H),
@@ -86,6 +98,17 @@ class HybridDecoder:
                 # cache: K transposed [N, kv, hd, T], V [N, kv, T, hd]; random history below each ctx
                 L.kt = torch.randn(n_slots, kv, hd, self.max_ctx, generator=g_, device=device).to(bf)
                 L.v = torch.randn(n_slots, kv, self.max_ctx, hd, generator=g_, device=device).to(bf)
+                L.cache = L.prefix = None
+                if cache_dtype is not None:
+                    L.cache = KVCache.empty(n_slots, kv, hd, self.max_ctx, cache_dtype, device)
+                    k, v = L.kt.permute(0, 3, 1, 2), L.v.transpose(1, 2)  # [slot, position, kv head, dim]
+                    kv_cache_store(L.cache, k.reshape(-1, kv, hd), v.reshape(-1, kv, hd), list(range(n_slots)))
+                    L.kt = L.v = None
+                if prefix_ctx:
+                    k, v = (torch.randn(prefix_ctx, kv, hd, generator=g_, device=device).to(bf) for _ in range(2))
+                    L.prefix = SharedPrefix(KVCache.empty(1, kv, hd, prefix_ctx, cache_dtype, device), self.prefix_len,
+                                            self.prefix_of)
+                    kv_cache_store(L.prefix.cache, k, v, [0])
             else:
                 Hv, Hk, C = cfg.gdn_v_heads, cfg.gdn_k_heads, cfg.conv_dim
                 L.in_proj = w(C + Hv * D + 2 * Hv, H)  # in_proj_qkv | in_proj_z | in_proj_b | in_proj_a
@@ -111,8 +134,12 @@ class HybridDecoder:
         rd = int(hd * cfg.rotary_frac)
         self.rotary_dim = rd
         self.inv_freq = 1.0 / (cfg.rope_theta ** (torch.arange(0, rd, 2, device=device, dtype=torch.float32) / rd))
-        self.attn_work = (attn_decode_workspace(n_slots, cfg.attn_heads, hd, self.max_ctx, device)
-                          if any(L.full for L in self.layers) else None)
+        full = next((L for L in self.layers if L.full), None)
+        self.attn_work = None
+        if full is not None:
+            self.attn_work = (attn_decode_workspace(n_slots, cfg.attn_heads, hd, self.max_ctx, device) if full.cache is None
+                              else cached_attn_workspace(full.cache, cfg.attn_heads, full.prefix))
+        self.sample_work = None
 
     # -- layers ------------------------------------------------------------------------------
     def gdn(self, i, L, x, partial=False):
@@ -133,8 +160,12 @@ class HybridDecoder:
         proj = decode_linear_partial(x, L.qkv_p)   # per head q | gate, then k, then v: split-K partials
         # q/k norms, partial rotary, the cache writes at each slot's position, softmax attention and
         # the sigmoid gate: three HIP launches
-        o = gqa_decode_attention(proj, self.pos, L.q_norm, L.k_norm, self.inv_freq, L.kt, L.v, nh, kv, hd,
-                                 self.rotary_dim, cfg.eps, work=self.attn_work)
+        if L.cache is not None:
+            o = cached_decode_attention(proj, self.pos, L.q_norm, L.k_norm, self.inv_freq, L.cache, nh, self.rotary_dim,
+                                        cfg.eps, work=self.attn_work, prefix=L.prefix)
+        else:
+            o = gqa_decode_attention(proj, self.pos, L.q_norm, L.k_norm, self.inv_freq, L.kt, L.v, nh, kv, hd,
+                                     self.rotary_dim, cfg.eps, work=self.attn_work)
         return (decode_linear_partial if partial else decode_linear)(o, L.o_p)
 
     def mlp(self, L, x, partial=False):
@@ -166,23 +197,35 @@ class HybridDecoder:
         self.pos += 1
         return decode_linear(x, self.lm_head_p) if self.lm_head_p is not None else x
 
+    def sample(self, logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        """The slots' next tokens (int64 [N]) from a step's logits and a random number per slot (sample_tokens, with the
+        decoder's workspace)."""
+        if self.sample_work is None:
+            self.sample_work = sample_workspace(self.N, logits.shape[1], logits.device)
+        return sample_tokens(logits, u, temperature, top_k, top_p, min_p, work=self.sample_work)
+
 
 class HybridDecodeGraph:
     """The whole decode step captured once as a HIP graph and replayed (src/cb_engine.py:123-187):
-    ``inp`` is the static input buffer, ``replay()`` returns the static output."""
+    ``inp`` is the static input buffer, ``replay()`` returns the static output.  With ``u`` (the static buffer of the
+    slots' random numbers) the step's tokens are drawn in the graph as well: ``tokens``, by ``sampling``'s temperature,
+    top_k, top_p and min_p (numbers, or static buffers with one per slot)."""
 
-    def __init__(self, model, inp):
-        self.model, self.inp = model, inp
+    def __init__(self, model, inp, u=None, **sampling):
+        self.model, self.inp, self.u = model, inp, u
         self.graph = torch.cuda.CUDAGraph()
         dev = inp.device
         stream = torch.cuda.Stream(device=dev)
         stream.wait_stream(torch.cuda.current_stream(dev))
         with torch.cuda.stream(stream):
-            model.step(inp)  # warm-up (advances the slots by one token)
+            logits = model.step(inp)  # warm-up (advances the slots by one token)
+            if u is not None:
+                model.sample(logits, u, **sampling)
         torch.cuda.current_stream(dev).wait_stream(stream)
         torch.cuda.synchronize(dev)
         with torch.cuda.graph(self.graph):
             self.out = model.step(inp)
+            self.tokens = None if u is None else model.sample(self.out, u, **sampling)
 
     def replay(self):
         self.graph.replay()
