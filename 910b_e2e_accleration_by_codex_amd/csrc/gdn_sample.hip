@@ -61,7 +61,9 @@ struct State {
   double target;    // top_p: the mass to reach
   int32_t left;     // top_k: the rank still to find in the bin
   int32_t quota;    // -1: no cut
-  int after_k;      // top_p's descent, behind top_k's
+  int k_level;      // top_p's descent, behind top_k's, which found so many digits (0: there was none)
+  uint32_t k_path;  // ... these
+  int cut_level;    // the cut's digits: all of them, or as many as set a bin apart that is kept whole
   uint32_t thr;     // the cut so far: keys above thr are kept, and the first `quota` elements with key thr
 };
 struct Hist {  // [N][S][BINS]
@@ -202,7 +204,9 @@ template <int W> struct Scratch {
   uint32_t count[W][BINS];  // each wave's share of the chunks
   double mass[W][BINS];
   State st;
-  double w;
+  double w;            // of the chosen bin: its value's weight (last digit), its mass, its elements
+  double bin_mass;
+  uint32_t bin_count;
 };
 // One digit: the row's chunks merged, and by the first wave the bin in which the cut lies (sc.st).  root: the descent's
 // first digit, whose masses are relative to the chunks' own maxima (top_p: of mass, its target's base; below 0: the row's
@@ -300,6 +304,8 @@ __device__ __forceinline__ void choose(const Hist& h, bool root, const Work& wk,
       st.prefix = st.prefix << 8 | (uint32_t)(4 * lane + hit);
       ++st.level;
       sc.st = st;
+      sc.bin_mass = hit == 0 ? m[0] : hit == 1 ? m[1] : hit == 2 ? m[2] : m[3];
+      sc.bin_count = hit == 0 ? c[0] : hit == 1 ? c[1] : hit == 2 ? c[2] : c[3];
       sc.w = hit == 0 ? v[0] : hit == 1 ? v[1] : hit == 2 ? v[2] : v[3];
     }
   }
@@ -330,7 +336,9 @@ __device__ __forceinline__ void advance(const Job& J, const Work& wk, const Row&
       sc.st.target = 0;
       sc.st.left = r.k;
       sc.st.quota = -1;
-      sc.st.after_k = 0;
+      sc.st.k_level = 0;
+      sc.st.k_path = 0;
+      sc.st.cut_level = J.levels;
       sc.st.thr = 0;
     }
   }
@@ -341,27 +349,39 @@ __device__ __forceinline__ void advance(const Job& J, const Work& wk, const Row&
   for (int h = i - 1;;) {
     choose(wk.step[h], h == 0, wk, r, wt, n, J.S, J.levels, sc, base, w);
     State st = sc.st;
-    if (st.level < J.levels) {
-      if (!st.after_k || st.thr >> (32 - 8 * st.level - (32 - 8 * J.levels)) != st.prefix) return;
-      ++h;  // top_p's descent along top_k's
+    const bool full = st.level == J.levels;
+    // a bin that is kept whole (all of it is wanted, or its only element) needs no further digits: the cut lies below it
+    const bool whole = !full && st.prefix && (st.kind == 1 ? st.left == (int)sc.bin_count : h > 0 && sc.bin_count == 1);
+    if (!full && !whole) {
+      if (st.level >= st.k_level || st.k_path >> 8 * (st.k_level - st.level) != st.prefix) return;
+      h = st.level;  // top_p's descent along top_k's
       continue;
     }
     if (st.kind == 1) {
+      st.k_level = st.level;
+      st.k_path = st.prefix;
+      base = whole ? st.above + sc.bin_mass : st.above + (double)st.left * w;
+    }
+    if (whole) {
+      st.thr = st.prefix - 1;
+      st.quota = 0;
+    } else if (st.kind == 1) {
       st.thr = st.prefix;
       st.quota = st.left;
-      base = st.above + (double)st.quota * w;
-      st.kind = r.by_p ? 2 : 0;
-      st.after_k = r.by_p;
+    } else {
+      const double m = ceil((st.target - st.above) / w);
+      const int32_t q = m >= 1.0 ? m < 2e9 ? (int32_t)m : INT32_MAX : 1;
+      const bool same = st.quota >= 0 && st.cut_level == J.levels && st.thr == st.prefix;  // as top_k's cut
+      st.quota = same && st.quota < q ? st.quota : q;
+      st.thr = st.prefix;
+    }
+    st.cut_level = st.level;
+    st.kind = st.kind == 1 && r.by_p ? 2 : 0;
+    if (st.kind) {
       st.level = 0;
       st.prefix = 0;
       st.above = 0;
       h = 0;
-    } else {
-      const double m = ceil((st.target - st.above) / w);
-      const int32_t q = m >= 1.0 ? m < 2e9 ? (int32_t)m : INT32_MAX : 1;
-      st.quota = st.quota >= 0 && st.thr == st.prefix && st.quota < q ? st.quota : q;
-      st.thr = st.prefix;
-      st.kind = 0;
     }
     __syncthreads();
     if (threadIdx.x == 0) sc.st = st;
@@ -481,7 +501,7 @@ __global__ __launch_bounds__(sample::TH, 4) void sample_pass_kernel(sample::Job 
   }
   // keys are compared up to the digits known: the prefix, or the whole cut (no cut: every key of a number is above 0)
   const Weights wt(r.t, st.M, table);
-  const int dsh = 24 - 8 * st.level, sh = count ? dsh + 8 : 32 - 8 * J.levels;
+  const int dsh = 24 - 8 * st.level, sh = count ? dsh + 8 : 32 - 8 * st.cut_level;
   const uint32_t ref = count ? st.prefix : st.quota >= 0 ? st.thr : 0;
   int64_t mass = 0;
   int ties = 0;
@@ -545,7 +565,7 @@ __global__ __launch_bounds__(sample::DT) void sample_draw_kernel(sample::Job J, 
     return;
   }
   const Weights weight(r.t, st.M, table);
-  const int sh = 32 - 8 * J.levels;
+  const int sh = 32 - 8 * st.cut_level;
   const bool cut = st.quota >= 0, open = was_kind;  // open: the waves' masses lack the bins of the last digit above the cut
   const uint32_t digit = st.thr & 255u;
   const int64_t quota = cut ? st.quota : 0;
