@@ -20,12 +20,13 @@ namespace gdn {
 namespace sample {
 constexpr int TH = 512;           // threads of a pass
 constexpr int EPT = 16;           // a thread's elements
-constexpr int CHUNK = TH * EPT;   // a row's elements per workgroup
+constexpr int CHUNK = TH * EPT;   // a row's elements per workgroup and turn
 constexpr int NW = TH / 64, WAVE = 64 * EPT;  // its waves, and their elements
 constexpr int BINS = 256;         // of a digit
 constexpr int COLS = 16;          // a bin's counters in LDS
 constexpr int DT = 512;           // threads of the draw
-constexpr int MOST = 1024 * CHUNK;  // logits of a row (the draw keeps its chunks in LDS)
+constexpr int MOST = 1024 * CHUNK;  // logits of a row (the draw keeps its workgroups' sums in LDS)
+constexpr int TURNS = 8;          // at most
 typedef unsigned long long u64;
 
 struct Params {  // per row (device), or NULL and one value for all
@@ -66,16 +67,16 @@ struct State {
   int cut_level;    // the cut's digits: all of them, or as many as set a bin apart that is kept whole
   uint32_t thr;     // the cut so far: keys above thr are kept, and the first `quota` elements with key thr
 };
-struct Hist {  // [N][S][BINS]
+struct Hist {  // [N][S][BINS], of the first pass [N][S0][BINS]
   uint32_t* count;
   u64* mass;
 };
 struct Work {
-  float* lmax;      // [N][S]: the chunks' maxima and their first indexes
+  float* lmax;      // [N][S0]: the chunks' maxima and their first indexes
   int32_t* larg;
   State* state;     // [2][N]
   Hist step[7];     // pass i's
-  int64_t* kept;    // [N][S][NW]: mass above the cut and elements at it, of each wave's elements
+  int64_t* kept;    // [N][S0 or more][NW]: mass above the cut and elements at it, of each wave's elements
   int32_t* ties;
 };
 struct Job {
@@ -85,9 +86,13 @@ struct Job {
   const double* u64_;
   int64_t* out;
   Params par;
-  int N, V, S, levels;
+  // a row's chunks; turns of a workgroup in the passes behind the first, and workgroups a row has in them
+  int N, V, S0, turns, S, levels;
   double one;  // the draw's weights: whole numbers of 1 / one
 };
+
+// The first element of workgroup s's turn, in the passes behind the first.
+__device__ __forceinline__ int64_t at_turn(const Job& J, int s, int turn) { return ((int64_t)s * J.turns + turn) * CHUNK; }
 
 // Order-preserving key of a value: -0 and 0 are equal, NaN is -inf.
 __device__ __forceinline__ float cleaned(float f) { return f != f ? -INFINITY : f + 0.f; }
@@ -325,7 +330,7 @@ __device__ __forceinline__ void advance(const Job& J, const Work& wk, const Row&
     if (threadIdx.x < sizeof(State) / 4) reinterpret_cast<uint32_t*>(&sc.st)[threadIdx.x] = from[threadIdx.x];
   } else if (threadIdx.x < 64) {
     float m = -INFINITY;
-    for (int s = threadIdx.x; s < J.S; s += 64) m = fmaxf(m, wk.lmax[(int64_t)n * J.S + s]);
+    for (int s = threadIdx.x; s < J.S0; s += 64) m = fmaxf(m, wk.lmax[(int64_t)n * J.S0 + s]);
     m = wave_max_fast(m);
     if (threadIdx.x == 0) {
       sc.st.M = m;
@@ -347,7 +352,7 @@ __device__ __forceinline__ void advance(const Job& J, const Work& wk, const Row&
   const Weights wt(r.t, sc.st.M, table);
   double base = -1.0, w;
   for (int h = i - 1;;) {
-    choose(wk.step[h], h == 0, wk, r, wt, n, J.S, J.levels, sc, base, w);
+    choose(wk.step[h], h == 0, wk, r, wt, n, h ? J.S : J.S0, J.levels, sc, base, w);
     State st = sc.st;
     const bool full = st.level == J.levels;
     // a bin that is kept whole (all of it is wanted, or its only element) needs no further digits: the cut lies below it
@@ -423,7 +428,7 @@ struct Counters {
 };
 }  // namespace sample
 
-// Pass 0, grid (S, N): the chunks' maxima, and the histogram of the first digit.
+// Pass 0, grid (S0, N): the chunks' maxima, and the histogram of the first digit.
 template <typename T>
 __global__ __launch_bounds__(sample::TH, 4) void sample_first_kernel(sample::Job J, sample::Work wk) {
   using namespace sample;
@@ -432,7 +437,7 @@ __global__ __launch_bounds__(sample::TH, 4) void sample_first_kernel(sample::Job
   __shared__ float tf[NW];
   __shared__ int first;
   const int n = blockIdx.y, s = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
-  const int64_t at = (int64_t)n * J.S + s;
+  const int64_t at = (int64_t)n * J.S0 + s;
   Chunk<T, EPT> c;
   c.load(static_cast<const T*>(J.logits) + n * J.stride, (int64_t)s * CHUNK + wid * WAVE, J.V);
   const Row r = row_of(J.par, n, J.V);
@@ -483,8 +488,9 @@ __global__ __launch_bounds__(sample::TH, 4) void sample_pass_kernel(sample::Job 
   __shared__ double table[64];
   const int n = blockIdx.y, s = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
   const int64_t at = (int64_t)n * J.S + s;
+  const T* row = static_cast<const T*>(J.logits) + n * J.stride;
   Chunk<T, EPT> c;
-  c.load(static_cast<const T*>(J.logits) + n * J.stride, (int64_t)s * CHUNK + wid * WAVE, J.V);
+  c.load(row, at_turn(J, s, 0) + wid * WAVE, J.V);
   const Row r = row_of(J.par, n, J.V);
   if (tid < 64) table[tid] = kPow[tid];
   advance(J, wk, r, n, i, table, lds.sc);
@@ -503,32 +509,35 @@ __global__ __launch_bounds__(sample::TH, 4) void sample_pass_kernel(sample::Job 
   const Weights wt(r.t, st.M, table);
   const int dsh = 24 - 8 * st.level, sh = count ? dsh + 8 : 32 - 8 * st.cut_level;
   const uint32_t ref = count ? st.prefix : st.quota >= 0 ? st.thr : 0;
-  int64_t mass = 0;
-  int ties = 0;
+  for (int turn = 0; turn < J.turns; ++turn) {
+    if (turn) c.load(row, at_turn(J, s, turn) + wid * WAVE, J.V);
+    int64_t mass = 0;
+    int ties = 0;
 #pragma unroll
-  for (int e = 0; e < EPT; ++e) {
-    const float v = c[e];
-    const uint32_t k = key_of(v), k1 = k >> sh;
-    const bool in = k1 == ref, above = last && k1 > ref && v != -INFINITY;
-    u64 w = 0;
-    if (above || (in && weigh)) {
-      const double x = wt(v);
-      w = fixed(x, above ? J.one : 0x1p50);
-      if (above && (x >= r.m || v == st.M)) mass += (int64_t)w;
+    for (int e = 0; e < EPT; ++e) {
+      const float v = c[e];
+      const uint32_t k = key_of(v), k1 = k >> sh;
+      const bool in = k1 == ref, above = last && k1 > ref && v != -INFINITY;
+      u64 w = 0;
+      if (above || (in && weigh)) {
+        const double x = wt(v);
+        w = fixed(x, above ? J.one : 0x1p50);
+        if (above && (x >= r.m || v == st.M)) mass += (int64_t)w;
+      }
+      if (in && count) {
+        const int b = (k >> dsh & 255u) * COLS + tid % COLS;
+        atomicAdd(&lds.h.count[b], 1u);
+        if (weigh) atomicAdd(&lds.h.mass[b], w);
+      }
+      ties += in;
     }
-    if (in && count) {
-      const int b = (k >> dsh & 255u) * COLS + tid % COLS;
-      atomicAdd(&lds.h.count[b], 1u);
-      if (weigh) atomicAdd(&lds.h.mass[b], w);
-    }
-    ties += in;
-  }
-  if (last) {
-    mass = wave_total(mass);
-    ties = wave_total(ties);
-    if (lane == 0) {
-      wk.kept[at * NW + wid] = mass;
-      wk.ties[at * NW + wid] = ties;
+    if (last) {
+      mass = wave_total(mass);
+      ties = wave_total(ties);
+      if (lane == 0) {
+        wk.kept[(at * J.turns + turn) * NW + wid] = mass;
+        wk.ties[(at * J.turns + turn) * NW + wid] = ties;
+      }
     }
   }
   if (!count) return;
@@ -536,18 +545,19 @@ __global__ __launch_bounds__(sample::TH, 4) void sample_pass_kernel(sample::Job 
   lds.h.write(wk.step[i], at, weigh);
 }
 
-// grid (N): the draw.  Sums of weights are whole numbers here: first over chunks, then over the found chunk's waves, then
-// over the found wave's elements.
+// grid (N): the draw.  Sums of weights are whole numbers here: first over the passes' workgroups, then over the found one's
+// waves and turns, then over the found wave's elements.
 template <typename T>
 __global__ __launch_bounds__(sample::DT) void sample_draw_kernel(sample::Job J, sample::Work wk, int passes) {
   using namespace sample;
   constexpr int W = DT / 64, MC = MOST / CHUNK, EW = WAVE / DT;
   __shared__ Scratch<W> sc;
   __shared__ double table[64];
-  __shared__ int64_t bin_mass[BINS], cmass[MC], wmass[NW], part[W], found_before, target_;
-  __shared__ int found, found_ties, cties[MC], wties[NW], tpart[W];
+  __shared__ int64_t bin_mass[BINS], cmass[MC], wmass[TURNS * NW], part[W], found_before, target_;
+  __shared__ int found, found_ties, cties[MC], wties[TURNS * NW], tpart[W];
   const int n = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
   const int64_t base = (int64_t)n * J.S;
+  const int nw = J.turns * NW;  // waves' sums of a workgroup
   const Row r = row_of(J.par, n, J.V);
   const int was_kind = wk.state[(int64_t)((passes - 1) & 1) * J.N + n].kind;
   double u = J.u64_ ? J.u64_[n] : (double)J.u[n];
@@ -558,8 +568,8 @@ __global__ __launch_bounds__(sample::DT) void sample_draw_kernel(sample::Job J, 
   if (r.greedy || st.M == -INFINITY) {
     if (tid == 0) found = INT32_MAX;
     __syncthreads();
-    for (int s = tid; s < J.S; s += DT)
-      if (wk.lmax[base + s] == st.M) atomicMin(&found, wk.larg[base + s]);
+    for (int s = tid; s < J.S0; s += DT)
+      if (wk.lmax[(int64_t)n * J.S0 + s] == st.M) atomicMin(&found, wk.larg[(int64_t)n * J.S0 + s]);
     __syncthreads();
     if (tid == 0) J.out[n] = st.M == -INFINITY ? -1 : found;
     return;
@@ -579,8 +589,8 @@ __global__ __launch_bounds__(sample::DT) void sample_draw_kernel(sample::Job J, 
   const int64_t wt = cut ? bin_mass[digit] : 0;
   const uint32_t* count = wk.step[passes - 1].count;
   for (int s = wid; s < J.S; s += W) {
-    int64_t m = lane < NW ? wk.kept[(base + s) * NW + lane] : 0;
-    int t = lane < NW && !open ? wk.ties[(base + s) * NW + lane] : 0;
+    int64_t m = lane < nw ? wk.kept[(base + s) * nw + lane] : 0;
+    int t = lane < nw && !open ? wk.ties[(base + s) * nw + lane] : 0;
     if (open) {
       const uint4 c4 = *reinterpret_cast<const uint4*>(count + (base + s) * BINS + 4 * lane);
       const uint32_t c[4] = {c4.x, c4.y, c4.z, c4.w};
@@ -627,9 +637,9 @@ __global__ __launch_bounds__(sample::DT) void sample_draw_kernel(sample::Job J, 
   if (found < 0) return;  // no mass: a row has its maximum at least, so this does not happen
   // ---- the chunk's waves
   const T* row = static_cast<const T*>(J.logits) + n * J.stride;
-  const int64_t c0 = (int64_t)found * CHUNK;
-  for (int x = wid; x < NW; x += W) {
-    const int64_t at = (base + found) * NW + x;
+  const int64_t c0 = at_turn(J, found, 0);
+  for (int x = wid; x < nw; x += W) {
+    const int64_t at = (base + found) * nw + x;
     int64_t m = 0;
     int t = 0;
     if (open) {
@@ -654,7 +664,7 @@ __global__ __launch_bounds__(sample::DT) void sample_draw_kernel(sample::Job J, 
   __syncthreads();
   int64_t upto = found_before;
   int before = found_ties, w0 = 0;
-  for (; w0 < NW - 1; ++w0) {
+  for (; w0 < nw - 1; ++w0) {
     const int64_t x = wties[w0], room = quota - before, in = room <= 0 ? 0 : x < room ? x : room;
     const int64_t y = wmass[w0] + in * wt;
     if (upto + y > target) break;
@@ -702,10 +712,9 @@ __global__ __launch_bounds__(sample::DT) void sample_draw_kernel(sample::Job J, 
 
 template <typename T>
 static int launch_sample(sample::Job J, const sample::Work& wk, bool by_k, bool by_p, hipStream_t st) {
-  const dim3 g(J.S, J.N);
   const int open = ((int)by_k + (int)by_p) * (J.levels - 1), passes = 1 + (open ? open : 1);
-  sample_first_kernel<T><<<g, sample::TH, 0, st>>>(J, wk);
-  for (int i = 1; i < passes; ++i) sample_pass_kernel<T><<<g, sample::TH, 0, st>>>(J, wk, i, passes);
+  sample_first_kernel<T><<<dim3(J.S0, J.N), sample::TH, 0, st>>>(J, wk);
+  for (int i = 1; i < passes; ++i) sample_pass_kernel<T><<<dim3(J.S, J.N), sample::TH, 0, st>>>(J, wk, i, passes);
   sample_draw_kernel<T><<<J.N, sample::DT, 0, st>>>(J, wk, passes);
   return check_launch("gdn_sample");
 }
@@ -714,9 +723,18 @@ static int launch_sample(sample::Job J, const sample::Work& wk, bool by_k, bool 
 using namespace gdn;
 
 namespace {
-int64_t sample_work(sample::Work& w, char* p, int N, int V) {
+// A row's chunks, and the turns its workgroups take in the passes behind the first: as few as let all of them be on the
+// chip at once (2 a CU), since each of them begins by merging its row's histograms.
+void sample_cut(sample::Job& J) {
+  J.S0 = (int)(((int64_t)J.V + sample::CHUNK - 1) / sample::CHUNK);
+  const int64_t t = ((int64_t)J.N * J.S0 + 511) / 512;
+  J.turns = t > sample::TURNS ? sample::TURNS : t < 1 ? 1 : (int)t;
+  J.S = (J.S0 + J.turns - 1) / J.turns;
+}
+int64_t sample_work(sample::Work& w, char* p, const sample::Job& J) {
   char* const base = p;
-  const int64_t S = ((int64_t)V + sample::CHUNK - 1) / sample::CHUNK, items = (int64_t)N * S;
+  const int N = J.N;
+  const int64_t items = (int64_t)N * J.S0, turns = (int64_t)N * J.S * J.turns;
   auto take = [&p](int64_t bytes) {
     char* q = p;
     p += (bytes + 255) / 256 * 256;
@@ -725,8 +743,8 @@ int64_t sample_work(sample::Work& w, char* p, int N, int V) {
   w.lmax = reinterpret_cast<float*>(take(items * 4));
   w.larg = reinterpret_cast<int32_t*>(take(items * 4));
   w.state = reinterpret_cast<sample::State*>(take(2ll * N * sizeof(sample::State)));
-  w.kept = reinterpret_cast<int64_t*>(take(items * sample::NW * 8));
-  w.ties = reinterpret_cast<int32_t*>(take(items * sample::NW * 4));
+  w.kept = reinterpret_cast<int64_t*>(take(turns * sample::NW * 8));
+  w.ties = reinterpret_cast<int32_t*>(take(turns * sample::NW * 4));
   for (sample::Hist& h : w.step) {
     h.mass = reinterpret_cast<sample::u64*>(take(items * sample::BINS * 8));
     h.count = reinterpret_cast<uint32_t*>(take(items * sample::BINS * 4));
@@ -737,8 +755,11 @@ int64_t sample_work(sample::Work& w, char* p, int N, int V) {
 
 extern "C" int64_t gdn_sample_workspace_bytes(int N, int V) {
   if (N < 0 || N > 65535 || V < 1 || V > sample::MOST) return -1;
+  sample::Job J{};
+  J.N = N, J.V = V;
+  sample_cut(J);
   sample::Work w;
-  return sample_work(w, nullptr, N, V);
+  return sample_work(w, nullptr, J);
 }
 
 extern "C" int gdn_sample(const void* logits, int64_t stride, int dtype, const void* u, int u_is_f64, const float* temperature,
@@ -758,17 +779,18 @@ extern "C" int gdn_sample(const void* logits, int64_t stride, int dtype, const v
   GDN_REQUIRE(temperature || (temperature1 >= -1e300 && temperature1 <= 1e300), "%s: the temperature must be finite", name);
   GDN_REQUIRE((top_p || (top_p1 >= 0.0 && top_p1 <= 1.0)) && (min_p || (min_p1 >= 0.0 && min_p1 <= 1.0)),
               "%s: top_p and min_p must be in [0, 1]", name);
-  sample::Work wk;
-  const int64_t need = sample_work(wk, static_cast<char*>(work), N, V);
-  GDN_REQUIRE(work_bytes >= need, "%s: workspace too small (%lld bytes needed)", name, (long long)need);
   sample::Job J{};
+  J.N = N, J.V = V;
+  sample_cut(J);
+  sample::Work wk;
+  const int64_t need = sample_work(wk, static_cast<char*>(work), J);
+  GDN_REQUIRE(work_bytes >= need, "%s: workspace too small (%lld bytes needed)", name, (long long)need);
   J.logits = logits;
   J.stride = stride;
   J.u = u_is_f64 ? nullptr : static_cast<const float*>(u);
   J.u64_ = u_is_f64 ? static_cast<const double*>(u) : nullptr;
   J.out = out;
   J.par = {temperature, top_p, min_p, top_k, temperature1, top_p1, min_p1, top_k1};
-  J.N = N, J.V = V, J.S = (int)(((int64_t)V + sample::CHUNK - 1) / sample::CHUNK);
   J.levels = dtype == GDN_BF16 ? 2 : dtype == GDN_F16 ? 3 : 4;
   J.one = 0x1p50;  // V weights of at most `one` stay below 2^62
   while (J.one > 1.0 && J.one * V > 0x1p62) J.one *= 0.5;
