@@ -95,7 +95,7 @@ struct Job {
 __device__ __forceinline__ int64_t at_turn(const Job& J, int s, int turn) { return ((int64_t)s * J.turns + turn) * CHUNK; }
 
 // Order-preserving key of a value: -0 and 0 are equal, NaN is -inf.
-__device__ __forceinline__ float cleaned(float f) { return f != f ? -INFINITY : f + 0.f; }
+__device__ __forceinline__ float cleaned(float f) { return fmaxf(f, -INFINITY) + 0.f; }
 __device__ __forceinline__ uint32_t key_of(float f) {
   const uint32_t b = __float_as_uint(f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
@@ -476,10 +476,10 @@ __global__ __launch_bounds__(sample::TH, 4) void sample_first_kernel(sample::Job
   if (count) lds.write(wk.step[0], at, r.by_p);
 }
 
-// Pass i >= 1 of `passes`, grid (S, N): the histogram of the next digit of the elements whose earlier digits are the prefix,
-// and in the last pass each wave's mass above the prefix, or above the cut and the elements at it where that is known.
-template <typename T>
-__global__ __launch_bounds__(sample::TH, 4) void sample_pass_kernel(sample::Job J, sample::Work wk, int i, int passes) {
+// Pass i >= 1, grid (S, N): the histogram of the next digit of the elements whose earlier digits are the prefix, and in the
+// last pass (kLast) each wave's mass above the prefix, or above the cut and the elements at it where that is known.
+template <typename T, bool kLast>
+__global__ __launch_bounds__(sample::TH, 4) void sample_pass_kernel(sample::Job J, sample::Work wk, int i) {
   using namespace sample;
   __shared__ union {
     Scratch<NW> sc;
@@ -497,10 +497,11 @@ __global__ __launch_bounds__(sample::TH, 4) void sample_pass_kernel(sample::Job 
   const State st = lds.sc.st;
   if (s == 0 && tid < (int)sizeof(State) / 4)
     reinterpret_cast<uint32_t*>(wk.state + (int64_t)(i & 1) * J.N + n)[tid] = reinterpret_cast<const uint32_t*>(&lds.sc.st)[tid];
-  const bool last = i == passes - 1, count = st.kind;
-  if (r.greedy || st.M == -INFINITY || !(count || last)) return;
+  const bool count = st.kind;
+  if (r.greedy || st.M == -INFINITY || !(count || kLast)) return;
   __syncthreads();
-  const bool weigh = count && r.by_p && st.level < J.levels - 1;
+  // (in the last pass the digit, if any, is the last one: a bin is one value, and needs no mass)
+  const bool weigh = !kLast && r.by_p && st.level < J.levels - 1;
   if (count) {
     lds.h.clear();
     __syncthreads();
@@ -517,21 +518,20 @@ __global__ __launch_bounds__(sample::TH, 4) void sample_pass_kernel(sample::Job 
     for (int e = 0; e < EPT; ++e) {
       const float v = c[e];
       const uint32_t k = key_of(v), k1 = k >> sh;
-      const bool in = k1 == ref, above = last && k1 > ref && v != -INFINITY;
-      u64 w = 0;
-      if (above || (in && weigh)) {
+      if (kLast && k1 > ref && v != -INFINITY) {
         const double x = wt(v);
-        w = fixed(x, above ? J.one : 0x1p50);
-        if (above && (x >= r.m || v == st.M)) mass += (int64_t)w;
+        if (x >= r.m || v == st.M) mass += (int64_t)fixed(x, J.one);
       }
-      if (in && count) {
-        const int b = (k >> dsh & 255u) * COLS + tid % COLS;
-        atomicAdd(&lds.h.count[b], 1u);
-        if (weigh) atomicAdd(&lds.h.mass[b], w);
+      if (k1 == ref) {
+        ++ties;
+        if (count) {
+          const int b = (k >> dsh & 255u) * COLS + tid % COLS;
+          atomicAdd(&lds.h.count[b], 1u);
+          if (weigh) atomicAdd(&lds.h.mass[b], fixed(wt(v), 0x1p50));
+        }
       }
-      ties += in;
     }
-    if (last) {
+    if (kLast) {
       mass = wave_total(mass);
       ties = wave_total(ties);
       if (lane == 0) {
@@ -714,7 +714,9 @@ template <typename T>
 static int launch_sample(sample::Job J, const sample::Work& wk, bool by_k, bool by_p, hipStream_t st) {
   const int open = ((int)by_k + (int)by_p) * (J.levels - 1), passes = 1 + (open ? open : 1);
   sample_first_kernel<T><<<dim3(J.S0, J.N), sample::TH, 0, st>>>(J, wk);
-  for (int i = 1; i < passes; ++i) sample_pass_kernel<T><<<dim3(J.S, J.N), sample::TH, 0, st>>>(J, wk, i, passes);
+  const dim3 g(J.S, J.N);
+  for (int i = 1; i < passes - 1; ++i) sample_pass_kernel<T, false><<<g, sample::TH, 0, st>>>(J, wk, i);
+  sample_pass_kernel<T, true><<<g, sample::TH, 0, st>>>(J, wk, passes - 1);
   sample_draw_kernel<T><<<J.N, sample::DT, 0, st>>>(J, wk, passes);
   return check_launch("gdn_sample");
 }
