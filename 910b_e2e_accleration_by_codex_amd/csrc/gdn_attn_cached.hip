@@ -7,7 +7,7 @@
 //   out = o sigmoid(gate).
 // Launches:
 //   1. cached_prep_kernel: a wave per (slot, head row).  Norm, rotary (angles in double), q to the workspace, k and v
-//      quantised into the cache.  One more wave plans: it sorts the slots by prefix into tiles of 32 query rows, and cuts
+//      quantised into the cache.  A few more workgroups plan: they sort the slots by prefix into tiles of 32 query rows, and cut
 //      every slot's own tokens and every tile's prefix into ranges of like cost, a workgroup each.
 //   2. cached_split_kernel: partial softmax sums of a range of tokens for 16 query rows (the G heads of one slot's kv
 //      head) or 32 (a tile of a prefix's slots).
@@ -165,17 +165,50 @@ __device__ __forceinline__ Slot slot_of(const Args& A, int n) {
 }
 __device__ __forceinline__ int blocks(int64_t tokens) { return (int)((tokens + BT - 1) / BT); }
 struct PlanLds {
-  int tokens[MAXN], prefix[MAXN], first[MAXN + 1];
-  int count[MAXP], tile[MAXP + 1], order[MAXP];  // a prefix's slots, first tile, place in order
+  alignas(16) int prefix[MAXN];
+  int tokens[MAXN], first[MAXN + 1];
+  // a prefix's slots, tokens, first tile, place in order, first range of all its tiles
+  int count[MAXP], len[MAXP], tile[MAXP + 1], order[MAXP + 1], part[MAXP + 1];
   unsigned long long cost;
-  int own, pre, tiles, wave[4];
+  int own, pre, wave[4];
 };
-// One workgroup of 256 threads.  Ranges cost the same: a block of a tile, with twice the query rows, counts as two of a
+// The sum of x over the threads before this one (256 threads; s.wave is free before and after).
+__device__ __forceinline__ int before(int x, PlanLds& s) {
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+  int up = x;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(up, o, kWave);
+    if (lane >= o) up += y;
+  }
+  if (lane == 63) s.wave[wid] = up;
+  __syncthreads();
+  int at = up - x;
+  for (int w = 0; w < wid; ++w) at += s.wave[w];
+  __syncthreads();
+  return at;
+}
+// The last entry that is at most f, of n ascending ones that begin with 0 (where several are alike, all but the last are of
+// something empty).
+__device__ __forceinline__ int entry_of(const int* first, int n, int f) {
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) / 2;
+    if (first[mid] <= f) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+// Workgroups of 256 threads, each of which finds the ranges and writes its share of the plan.  Ranges cost the same: a block of a tile, with twice the query rows, counts as two of a
 // slot's own.  Ranges are whole turns of a workgroup's waves.
-__device__ __forceinline__ void make_plan(const Args& A, const Work& wk, PlanLds& s) {
-  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, G = A.nh / A.nkv;
+__device__ __forceinline__ void make_plan(const Args& A, const Work& wk, int planner, int planners, PlanLds& s) {
+  const int tid = threadIdx.x, G = A.nh / A.nkv;
+  const int i0 = planner * 256 + tid, step = planners * 256;  // of what is written
   if (tid == 0) s.cost = 0;
-  for (int r = tid; r < A.P; r += 256) s.count[r] = 0;
+  for (int r = tid; r < A.P; r += 256) {
+    s.count[r] = 0;
+    s.len[r] = (int)prefix_len(A, r);
+  }
   __syncthreads();
   unsigned long long cost = 0;
   for (int n = tid; n < A.N; n += 256) {
@@ -185,93 +218,96 @@ __device__ __forceinline__ void make_plan(const Args& A, const Work& wk, PlanLds
     cost += blocks(x.own);
     if (x.prefix >= 0) atomicAdd(&s.count[x.prefix], 1);
   }
+  __syncthreads();
+  // thread t's prefixes are r0 .. r1 - 1, its slots n0 .. n1 - 1
+  const int rp = (A.P + 255) / 256, r0 = tid * rp, r1 = r0 + rp < A.P ? r0 + rp : A.P;
+  const int np = (A.N + 255) / 256, n0 = tid * np, n1 = n0 + np < A.N ? n0 + np : A.N;
+  auto tiles_of = [&](int r) { return (s.count[r] * G + PROWS - 1) / PROWS; };
+  if (A.P) {
+    int sum = 0;  // tiles, at most 1536, times 65536, and slots
+    for (int r = r0; r < r1; ++r) {
+      sum += tiles_of(r) << 16 | s.count[r];
+      cost += 2ull * tiles_of(r) * blocks(s.len[r]);
+    }
+    sum = before(sum, s);
+    for (int r = r0; r < r1; ++r) {
+      s.tile[r] = sum >> 16, s.order[r] = sum & 0xffff;
+      sum += tiles_of(r) << 16 | s.count[r];
+    }
+    if (r0 < r1 && r1 == A.P) s.tile[A.P] = sum >> 16;
+  }
   if (cost) atomicAdd(&s.cost, cost);
   __syncthreads();
   if (tid == 0) {
-    int tile = 0, order = 0;
-    unsigned long long c = s.cost;
-    for (int r = 0; r < A.P; ++r) {
-      const int nt = (s.count[r] * G + PROWS - 1) / PROWS;
-      s.tile[r] = tile, s.order[r] = order;
-      tile += nt, order += s.count[r];
-      if (nt) c += 2ull * nt * blocks(prefix_len(A, r));
-    }
-    s.tile[A.P] = tile;
     // a workgroup a CU; of slots' own tokens, which HBM bounds, 4 that even out where there are many blocks (16 slots of
     // 16384 to 32768 tokens: 199 us with one, 154 with four; 64 slots behind 16384 shared tokens: 105 us with four, 91)
-    unsigned long long each = (c + WGS / A.nkv) / (WGS / A.nkv + 1);
+    unsigned long long each = (s.cost + WGS / A.nkv) / (WGS / A.nkv + 1);
     if (each > 1 << 28) each = 1 << 28;
     s.pre = (int)((each + 2 * WAVES - 1) / (2 * WAVES)) * WAVES;
     if (each >= 4 * LONG) each = (each + 3) / 4;
     s.own = (int)((each + WAVES - 1) / WAVES) * WAVES;
   }
   __syncthreads();
-  // the slots' ranges: thread t's slots are t * per ..
-  const int per = (A.N + 255) / 256;
-  int mine = 0;
-  for (int n = tid * per; n < (tid + 1) * per && n < A.N; ++n) mine += s.own ? (blocks(s.tokens[n]) + s.own - 1) / s.own : 0;
-  int up = mine;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(up, o, kWave);
-    if (lane >= o) up += y;
-  }
-  if (lane == 63) s.wave[wid] = up;
-  __syncthreads();
-  int at = up - mine;
-  for (int w = 0; w < wid; ++w) at += s.wave[w];
-  for (int n = tid * per; n < (tid + 1) * per && n < A.N; ++n) {
+  // ranges of a slot, and of one tile of a prefix
+  auto own_of = [&](int n) { return s.own ? (blocks(s.tokens[n]) + s.own - 1) / s.own : 0; };
+  auto pre_of = [&](int r) { return s.pre && s.count[r] ? (blocks(s.len[r]) + s.pre - 1) / s.pre : 0; };
+  int sum = 0;  // ranges of slots, at most 5 WGS + MAXN, times 65536, and of tiles
+  for (int n = n0; n < n1; ++n) sum += own_of(n) << 16;
+  for (int r = r0; r < r1; ++r) sum += pre_of(r) * tiles_of(r);
+  sum = before(sum, s);
+  int at = sum >> 16, part = sum & 0xffff;
+  for (int n = n0; n < n1; ++n) {
     s.first[n] = at;
-    at += s.own ? (blocks(s.tokens[n]) + s.own - 1) / s.own : 0;
+    at += own_of(n);
   }
-  if (tid == 0) s.first[A.N] = s.wave[0] + s.wave[1] + s.wave[2] + s.wave[3];
+  if (n0 < n1 && n1 == A.N) s.first[A.N] = at;
+  for (int r = r0; r < r1; ++r) {
+    s.part[r] = part;
+    part += pre_of(r) * tiles_of(r);
+  }
+  if (r0 < r1 && r1 == A.P) s.part[A.P] = part;
   __syncthreads();
-  for (int n = tid; n < A.N; n += 256) {
+  for (int n = i0; n < A.N; n += step) {
     SlotPlan p{s.first[n], s.first[n + 1] - s.first[n], -1, 0};
     const int r = s.prefix[n];
     if (r >= 0) {
       p.tile = s.tile[r];
-      for (int m = 0; m < n; ++m) p.rank += s.prefix[m] == r;
+#pragma unroll 4
+      for (int m = 0; m < n; m += 4) {
+        const int4 x = *reinterpret_cast<const int4*>(&s.prefix[m]);
+        p.rank += (x.x == r) + (m + 1 < n && x.y == r) + (m + 2 < n && x.z == r) + (m + 3 < n && x.w == r);
+      }
       wk.order[s.order[r] + p.rank] = n;
     }
     wk.slots[n] = p;
   }
   // ---- prefixes first, as they are the longest.  A range's tiles lie 8 workgroups apart: on one XCD, whose L2 then
   // has the range's keys and values for all of them
-  int item = 0, part = 0;
-  for (int r = 0; r < A.P; ++r) {
-    const int t0 = s.tile[r], nt = s.tile[r + 1] - t0, rows = s.count[r] * G;
-    if (!nt) continue;
-    const int tokens = (int)prefix_len(A, r), n = blocks(tokens), parts = n ? (n + s.pre - 1) / s.pre : 0;
-    for (int t = tid; t < nt; t += 256) {
-      const int left = rows - t * PROWS;
-      wk.tiles[t0 + t] = TilePlan{r, s.order[r], t * PROWS, left < PROWS ? left : PROWS, part + t * parts, parts, {0, 0}};
+  int item = 0;
+  if (A.P) {
+    for (int t = i0; t < s.tile[A.P]; t += step) {
+      const int r = entry_of(s.tile, A.P, t), in = t - s.tile[r], left = s.count[r] * G - in * PROWS, parts = pre_of(r);
+      wk.tiles[t] = TilePlan{r, s.order[r], in * PROWS, left < PROWS ? left : PROWS, s.part[r] + in * parts, parts, {0, 0}};
     }
-    const int units = parts * A.nkv;
-    for (int i = tid; i < units * nt; i += 256) {
-      const int group = i / (8 * nt), in = i % (8 * nt), left = units - 8 * group, w = left < 8 ? left : 8;
-      const int t = in / w, u = 8 * group + in % w, p = u / A.nkv;
-      const int end = (p + 1) * s.pre;
-      wk.items[item + i] = Item{t0 + t, r, u % A.nkv, p * s.pre, end < n ? end : n, tokens, part + t * parts + p, 0};
+    item = s.part[A.P] * A.nkv;
+    for (int i = i0; i < item; i += step) {
+      const int r = entry_of(s.part, A.P, i / A.nkv), nt = tiles_of(r), parts = pre_of(r), units = parts * A.nkv;
+      const int x = i - s.part[r] * A.nkv, group = x / (8 * nt), in = x % (8 * nt);
+      const int left = units - 8 * group, w = left < 8 ? left : 8;
+      const int t = in / w, u = 8 * group + in % w, p = u / A.nkv, end = (p + 1) * s.pre;
+      const int nb = blocks(s.len[r]);
+      wk.items[i] = Item{s.tile[r] + t, r, u % A.nkv, p * s.pre, end < nb ? end : nb, s.len[r], s.part[r] + t * parts + p, 0};
     }
-    item += units * nt;
-    part += parts * nt;
   }
   // ---- the slots' own tokens
   const int own = s.first[A.N] * A.nkv;
-  for (int i = tid; item + i < A.items; i += 256) {
+  for (int i = i0; item + i < A.items; i += step) {
     Item x{-1, 0, 0, 0, 0, 0, 0, 0};
     if (i < own) {
-      const int f = i / A.nkv;
-      int lo = 0, hi = A.N - 1;  // the last slot that begins at f or before (an empty one begins where the next does)
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) / 2;
-        if (s.first[mid] <= f) lo = mid;
-        else hi = mid - 1;
-      }
-      const int n = blocks(s.tokens[lo]), np = s.first[lo + 1] - s.first[lo], in = i - s.first[lo] * A.nkv;
-      const int p = in % np, end = (p + 1) * s.own;
-      x = Item{-1, lo, in / np, p * s.own, end < n ? end : n, s.tokens[lo], s.first[lo] + p, 0};
+      const int f = i / A.nkv, n = entry_of(s.first, A.N, f);
+      const int nb = blocks(s.tokens[n]), parts = s.first[n + 1] - s.first[n], in = i - s.first[n] * A.nkv;
+      const int p = in % parts, end = (p + 1) * s.own;
+      x = Item{-1, n, in / parts, p * s.own, end < nb ? end : nb, s.tokens[n], s.first[n] + p, 0};
     }
     wk.items[item + i] = x;
   }
@@ -286,9 +322,9 @@ template <int HD, int RT> struct SplitLds {
 };
 }  // namespace cached
 
-// A wave per (slot, row), rows: nh query heads, nkv keys, nkv values; lane l holds dims l + 64 e.  The last workgroup plans.
+// A wave per (slot, row), rows: nh query heads, nkv keys, nkv values; lane l holds dims l + 64 e.  The first workgroups plan.
 template <int HD, bool F8>
-__global__ __launch_bounds__(256) void cached_prep_kernel(cached::Args A, cached::Work wk) {
+__global__ __launch_bounds__(256) void cached_prep_kernel(cached::Args A, cached::Work wk, int planners) {
   using namespace cached;
   constexpr int E = HD / 64;
   __shared__ union {
@@ -297,12 +333,12 @@ __global__ __launch_bounds__(256) void cached_prep_kernel(cached::Args A, cached
   } lds;
   auto& tmp = lds.tmp;
   const int wid = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  if (blockIdx.x == gridDim.x - 1) {
-    make_plan(A, wk, lds.plan);
+  if ((int)blockIdx.x < planners) {
+    make_plan(A, wk, blockIdx.x, planners, lds.plan);
     return;
   }
   const int per = A.nh + 2 * A.nkv;
-  const int64_t w = (int64_t)blockIdx.x * 4 + wid;
+  const int64_t w = (int64_t)(blockIdx.x - planners) * 4 + wid;
   if (w >= (int64_t)A.N * per) return;  // whole waves: no barrier below
   const int n = (int)(w / per), r = (int)(w % per);
   const bool is_q = r < A.nh, is_v = r >= A.nh + A.nkv;
@@ -728,7 +764,8 @@ template <int HD, bool F8>
 static int launch_cached(const cached::Args& A, const cached::Work& wk, hipStream_t st) {
   const int64_t waves = (int64_t)A.N * (A.nh + 2 * A.nkv);
   const float scale2 = 1.4426950408889634f / sqrtf((float)HD);  // scores in powers of two
-  cached_prep_kernel<HD, F8><<<(unsigned)((waves + 3) / 4 + 1), 256, 0, st>>>(A, wk);
+  const int planners = A.items < 8 * 256 ? (A.items + 255) / 256 : 8;
+  cached_prep_kernel<HD, F8><<<(unsigned)((waves + 3) / 4 + planners), 256, 0, st>>>(A, wk, planners);
   if (A.pof) cached_split_kernel<HD, F8, true><<<A.items, 256, 0, st>>>(A, wk, scale2);
   else cached_split_kernel<HD, F8, false><<<A.items, 256, 0, st>>>(A, wk, scale2);
   cached_combine_kernel<HD><<<A.N * A.nh, 256, 0, st>>>(A, wk);

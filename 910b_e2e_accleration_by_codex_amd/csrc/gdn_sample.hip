@@ -730,13 +730,15 @@ namespace {
 void sample_cut(sample::Job& J) {
   J.S0 = (int)(((int64_t)J.V + sample::CHUNK - 1) / sample::CHUNK);
   const int64_t t = ((int64_t)J.N * J.S0 + 511) / 512;
-  J.turns = t > sample::TURNS ? sample::TURNS : t < 1 ? 1 : (int)t;
+  const int most = J.S0 < sample::TURNS ? J.S0 : sample::TURNS;
+  J.turns = t > most ? most : t < 1 ? 1 : (int)t;
   J.S = (J.S0 + J.turns - 1) / J.turns;
 }
 int64_t sample_work(sample::Work& w, char* p, const sample::Job& J) {
   char* const base = p;
   const int N = J.N;
-  const int64_t items = (int64_t)N * J.S0, turns = (int64_t)N * J.S * J.turns;
+  // (J.S * J.turns may be less for more rows; a workspace for many rows has to hold fewer)
+  const int64_t items = (int64_t)N * J.S0, turns = (int64_t)N * (J.S0 + sample::TURNS - 1);
   auto take = [&p](int64_t bytes) {
     char* q = p;
     p += (bytes + 255) / 256 * 256;

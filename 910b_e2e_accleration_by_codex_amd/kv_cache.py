@@ -176,7 +176,7 @@ def kv_cache_load(cache, rows, cu_seqlens, start=None, total_tokens=None):
     """The keys and values that a cache holds, as packed bf16 rows: sequence s gives positions start[s] .. start[s] +
     (cu_seqlens[s + 1] - cu_seqlens[s]) - 1 of row rows[s].  Arguments as kv_cache_store; with cu_seqlens on the device give
     ``total_tokens`` (its last entry) too, or it is read back.  Returns (k, v) [total_tokens, kv, hd] bf16; positions and
-    rows outside the cache are zeros."""
+    rows outside the cache are zeros, and tokens that no sequence covers (behind the last one of a padded batch) hold anything."""
     name = "kv_cache_load"
     code, R, kv, hd, T, _ = _check(name, cache)
     dev = cache.k.device
@@ -239,7 +239,7 @@ def cached_decode_attention(proj, pos, q_norm, k_norm, inv_freq, cache, n_heads,
             or (rotary_dim and inv_freq.get_device() != dev):
         _lib.require_cuda(proj, pos, q_norm, k_norm)
         raise ValueError(f"{name}: every tensor must be on the cache's device {cache.k.device}")
-    if part is None and proj.stride(1) != 1:
+    if part is None and (proj.stride(1) != 1 or (N > 1 and proj.stride(0) < width)):
         proj = proj.contiguous()
     P, Tp, pre = 0, 0, _NO_PREFIX
     if prefix is not None:

@@ -19,8 +19,12 @@ def _param(what, x, N, dtype, device):
     """(device pointer or None, value): a number for every row, or a tensor [N] on the device."""
     if not isinstance(x, torch.Tensor):
         return None, x, None
+    if dtype is torch.int32 and (x.dtype.is_floating_point or x.dtype is torch.bool):
+        raise TypeError(f"sample_tokens: {what} must be whole numbers, got {x.dtype}")
     if not x.is_cuda or x.device != device or x.numel() != N:
         raise ValueError(f"sample_tokens: {what} must be a number or a tensor of {N} entries on {device}")
+    if x.dtype is torch.int64 and dtype is torch.int32:
+        x = x.clamp(-1, 2 ** 31 - 1)
     x = x.reshape(-1).to(dtype).contiguous()
     return x.data_ptr(), 0, x
 
@@ -48,11 +52,13 @@ def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, wor
                             ("top_k", top_k, -2 ** 31, 2 ** 31 - 1)):
         if not isinstance(x, torch.Tensor) and not lo <= x <= hi:
             raise ValueError(f"sample_tokens: {what} = {x} is outside [{lo}, {hi}]")
+    if not isinstance(top_k, torch.Tensor) and int(top_k) != top_k:
+        raise TypeError(f"sample_tokens: top_k must be a whole number, got {top_k}")
     t, t1, keep_t = _param("temperature", temperature, N, torch.float32, dev)
     k, k1, keep_k = _param("top_k", top_k, N, torch.int32, dev)
     p, p1, keep_p = _param("top_p", top_p, N, torch.float32, dev)
     m, m1, keep_m = _param("min_p", min_p, N, torch.float32, dev)
-    if logits.stride(1) != 1:
+    if logits.stride(1) != 1 or (N > 1 and logits.stride(0) < V):  # (one row for all, too)
         logits = logits.contiguous()
     u = u.contiguous()
     out = torch.empty(N, dtype=torch.int64, device=dev)

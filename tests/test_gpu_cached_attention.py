@@ -280,6 +280,40 @@ def test_other_stream_and_strided_projection(gdn, dev):
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("N,P", [(400, 300), (1024, 1024), (1024, 3)])
+def test_many_slots_and_prefixes(gdn, dev, N, P):
+    """As many slots and prefixes as a call takes; prefixes without slots, slots without a prefix, empty prefixes."""
+    nh, kv, hd, T, Tp = 2, 1, 64, 64, 128
+    g = torch.Generator().manual_seed(N + P)
+    x, px = make(N, nh, kv, hd, T, True, N), make(P, nh, kv, hd, Tp, True, P)
+    plen = torch.randint(0, Tp + 1, (P,), generator=g)
+    of = torch.randint(-1, P + 1, (N,), generator=g)
+    full = torch.where((of >= 0) & (of < P), plen[of.clamp(0, P - 1)], 0)
+    pos = full + torch.randint(0, T, (N,), generator=g)
+    prefix = gdn.SharedPrefix(on_gpu(gdn, px, dev), plen.int().to(dev), of.int().to(dev))
+    out, c = run(gdn, dev, x, pos.tolist(), nh, prefix)
+    p = (so.unpack(px["k"], px["ke"], "k"), so.unpack(px["v"], px["ve"], "v"), plen.tolist(), of.tolist())
+    ref, raw, k, v = reference(x, pos.tolist(), nh, True, p)
+    for n in range(N):
+        assert rel_l2(out[n], ref[n]) <= TOL, n
+    check_cache(c, x, k, v, raw, (pos - full).tolist(), T)
+
+
+def test_one_projection_for_all_slots_and_no_slots(gdn, dev):
+    nh, kv, hd, T, N = 4, 2, 64, 64, 5
+    x = make(N, nh, kv, hd, T, False, 14)
+    x["proj"] = x["proj"][:1].expand(N, -1)
+    pos = [0, 3, 9, 40, 63]
+    c = on_gpu(gdn, x, dev)
+    args = (torch.tensor(pos, device=dev), x["qn"].to(dev), x["kn"].to(dev), x["inv"].to(dev))
+    out = gdn.cached_decode_attention(x["proj"][:1].to(dev).expand(N, -1), *args, c, nh, x["rd"], EPS)
+    ref, _, _, _ = reference(x, pos, nh, False)
+    for n in range(N):
+        assert rel_l2(out[n], ref[n]) <= TOL, pos[n]
+    none = gdn.KVCache(c.k[:0], c.v[:0])
+    assert gdn.cached_decode_attention(x["proj"][:0].to(dev), args[0][:0], *args[1:], none, nh, x["rd"], EPS).shape == (0, nh * hd)
+
+
 def test_refusals(gdn, dev):
     nh, kv, hd, N = 4, 2, 64, 2
     x = make(N, nh, kv, hd, 64, True, 13)

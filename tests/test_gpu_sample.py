@@ -116,6 +116,36 @@ def test_graph_and_stream(gdn, dev):
     assert torch.equal(got2, got)
 
 
+@pytest.mark.parametrize("dtype,N,V", [(BF, 600, 20000), (torch.float32, 700, 9000), (torch.float16, 2500, 100), (torch.float32, 2, 1000003)])
+def test_many_rows_and_long_ones(gdn, dev, dtype, N, V):
+    """Rows of which a workgroup takes several chunks, rows shorter than that, and a row of many chunks; the workspace of
+    these rows serves fewer as well."""
+    l, u = logits_of(N, V, dtype, N)
+    work = gdn.sample_workspace(N, V, dev)
+    ld, ud = l.to(dev), u.to(dev)
+    for par in ((1.0, 0, 1.0, 0.0), (0.9, 40, 0.9, 0.01)):
+        want = so.sample(l, u.numpy(), *par)
+        assert torch.equal(gdn.sample_tokens(ld, ud, *par, work=work).cpu(), want)
+        n = N // 2
+        assert torch.equal(gdn.sample_tokens(ld[:n], ud[:n], *par, work=work).cpu(), want[:n])
+
+
+def test_one_row_for_all_and_wide_parameters(gdn, dev):
+    """The same logits for every random number (a row stride of 0), an odd row start, and top_k in int64 past 32 bits."""
+    l, u = logits_of(1, 5001, BF, 30)
+    u = torch.rand(64, generator=torch.Generator().manual_seed(1), dtype=torch.float64)
+    want = so.sample(l.expand(64, -1), u.numpy(), 1.0, 0, 0.9, 0.0)
+    assert torch.equal(gdn.sample_tokens(l.to(dev).expand(64, -1), u.to(dev), 1.0, 0, 0.9).cpu(), want)
+    l, u = logits_of(4, 3001, torch.float32, 31)
+    k = torch.tensor([2 ** 32 + 5, 2 ** 31, -(2 ** 40), 5], device=dev)
+    got = gdn.sample_tokens(l.to(dev)[:, 1:], u.to(dev), 1.0, k)
+    assert torch.equal(got.cpu(), so.sample(l[:, 1:], u.numpy(), 1.0, [0, 0, 0, 5], 1.0, 0.0))
+    with pytest.raises(TypeError, match="whole"):
+        gdn.sample_tokens(l.to(dev), u.to(dev), 1.0, 2.5)
+    with pytest.raises(TypeError, match="whole"):
+        gdn.sample_tokens(l.to(dev), u.to(dev), 1.0, k.float())
+
+
 def test_refusals(gdn, dev):
     l, u = torch.zeros(2, 10, device=dev), torch.zeros(2, device=dev)
     for args, kw in (((l[0], u), {}), ((l, u[:1]), {}), ((l, u.half()), {}), ((l, u, float("nan")), {}), ((l, u, float("inf")), {}),

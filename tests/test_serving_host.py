@@ -80,6 +80,21 @@ def test_c_abi_refuses(gdn):
     assert sample(N=0) == 0
 
 
+def test_c_abi_limits_and_workspaces(gdn):
+    """A call takes 1024 slots and prefixes and 8388608 logits a row; a workspace for many rows or slots holds fewer."""
+    h = importlib.import_module(PKG_NAME + "._lib").lib()
+    attn = lambda N, P=0, T=128, Tp=128: h.gdn_attn_cached_workspace_bytes(N, 24, 4, 256, T, P, Tp)  # noqa: E731
+    assert attn(1024, 1024) > 0 and attn(1025) == -1 and attn(4, 1025) == -1
+    sizes = [attn(n, 2, 32768, 16384) for n in range(0, 200)]
+    assert sizes == sorted(sizes)
+    assert h.gdn_sample_workspace_bytes(1, 8388608) > 0 and h.gdn_sample_workspace_bytes(1, 8388609) == -1
+    for V in (1, 9000, 65537, 131072, 248320):
+        sizes = [h.gdn_sample_workspace_bytes(n, V) for n in range(0, 1200)]
+        assert sizes == sorted(sizes)
+    sizes = [h.gdn_sample_workspace_bytes(500, v) for v in range(1, 300000, 997)]
+    assert sizes == sorted(sizes)
+
+
 def test_oracle_quantises_as_torch_does():
     """Codes are torch's own e4m3 rounding of x 2^-e, and e is the smallest that fits."""
     g = torch.Generator().manual_seed(1)
