@@ -12,10 +12,24 @@
 //   2. cached_split_kernel: partial softmax sums of a range of tokens for 16 query rows (the G heads of one slot's kv
 //      head) or 32 (a tile of a prefix's slots).
 //   3. cached_combine_kernel: per (slot, head) the partials merged by their maxima, and the gate.
-// Rounding: K and V enter as the cache holds them (e4m3 codes are bf16 values, their scales multiply scores and
-// probabilities in fp32).  The query and the probabilities are fp32 values that enter the bf16 products as a high and a low
-// part, two products each: one rounding of each to bf16 would nearly double the error of the rounded output (0.0031
-// against 0.0017 relative), and these products are not what bounds the kernel.  The output is rounded once, to bf16.
+// Rounding: K and V enter as the cache holds them (e4m3 codes are fp16 and bf16 values, their scales multiply scores and
+// probabilities in fp32).  The query against e4m3 keys is rounded to fp16 once, in units of its row's largest value, an
+// eighth of the output's rounding (with the two parts below 64 slots behind 16384 shared tokens take 81 us instead of 74).
+// The query against bf16 keys, and the probabilities, enter the bf16 products as a high and a low part, two products each:
+// one rounding of each to bf16 would nearly double the error of the rounded output (0.0031 against 0.0017 relative).  The
+// output is rounded once, to bf16.
+//
+// Measured, 24 query and 4 kv heads of 256 (a large read runs at 6.07 TB/s, a large bf16 product at 1374 TFLOP/s), the
+// kernels' medians in us:
+//                                               bytes    prep  split  combine  split's rate
+//   16 slots of 512 to 4096 tokens, e4m3       76 MB     4.8   17.8    4.0     4.3 TB/s
+//   the same, bf16                            152 MB     4.4   27.7    4.2     5.5 TB/s
+//   16 slots of 16384 to 32768 tokens, e4m3   809 MB     6.2  156      6.1     5.2 TB/s
+//   16 slots behind 8192 shared tokens, e4m3   35 MB     7.0   19.4    4.7     177 TFLOP/s
+//   64 slots behind 2 x 16384, e4m3           108 MB     9.8   74      5.4     354 TFLOP/s
+// Slots' own tokens are bound by HBM, and where few, by the latency of a workgroup's start and merge (7 us of the 17.8).
+// A prefix's tiles are bound by the vector instructions around the products (codes widened, the softmax, probabilities
+// split and scaled) at one wave a SIMD.
 #include "gdn_attn.h"
 #include "gdn_device.h"
 #include "gdn_internal.h"
@@ -30,7 +44,17 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
-// 8 e4m3 codes -> 8 bf16 values (exact).
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ f32x4 mma16(u32x4 a, u32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+// 8 e4m3 codes -> 8 fp16 values (exact), and 8 bf16 values (exact).
+__device__ __forceinline__ u32x4 widen16(uint32_t lo, uint32_t hi) {
+  return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false)),
+               __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true))};
+}
 __device__ __forceinline__ u32x4 widen(uint32_t lo, uint32_t hi) {
   return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false)),
                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true)),
@@ -99,10 +123,11 @@ struct TilePlan {
   int first, count;              // its partials
   int pad[2];
 };
-// workspace: q (fp32 [N, nh, hd]) | partials: m, l (fp32 [parts, 2]) and o (fp32 [parts, hd]), parts = own_parts * nkv * G of
+// workspace: q ([N, nh, hd] fp16 for an e4m3 cache, [N, nh, 2, hd] bf16 for a bf16 one), its rows' scales (fp32 [N, nh]) | partials: m, l (fp32 [parts, 2]) and o (fp32 [parts, hd]), parts = own_parts * nkv * G of
 // slots, then pre_parts * nkv * 32 of tiles | the plan
 struct Work {
-  float *q, *ml, *o;
+  uint16_t* q;
+  float *scale, *ml, *o;
   Item* items;
   SlotPlan* slots;
   TilePlan* tiles;
@@ -133,7 +158,8 @@ inline int64_t work_of(Work& w, char* p, const Args& A, int hd) {
     return q;
   };
   const int64_t parts = (int64_t)A.own_parts * A.nh + (int64_t)A.pre_parts * A.nkv * PROWS;
-  w.q = reinterpret_cast<float*>(take((int64_t)A.N * A.nh * hd * 4));
+  w.q = reinterpret_cast<uint16_t*>(take((int64_t)A.N * A.nh * hd * 4));
+  w.scale = reinterpret_cast<float*>(take((int64_t)A.N * A.nh * 4));
   w.ml = reinterpret_cast<float*>(take(parts * 8));
   w.o = reinterpret_cast<float*>(take(parts * hd * 4));
   w.items = reinterpret_cast<Item*>(take((int64_t)A.items * sizeof(Item)));
@@ -312,10 +338,11 @@ __device__ __forceinline__ void make_plan(const Args& A, const Work& wk, int pla
     wk.items[item + i] = x;
   }
 }
-template <int HD, int RT> struct SplitLds {
+template <int HD, bool F8, int RT> struct SplitLds {
+  static constexpr int PARTS = F8 ? 1 : 2;        // of q
   static constexpr int R = 16 * RT, LQ = HD + 8;  // query rows, and their pitch
   static constexpr int DS = 64;                   // dims per round of the merge
-  alignas(16) uint16_t qs[2][R * LQ];
+  alignas(16) uint16_t qs[PARTS][R * LQ];
   alignas(16) float so[WAVES][R][DS + 4];
   float sm[WAVES][R], sl[WAVES][R];
   int rown[R], rowh[R];  // each row's slot (-1: none) and head
@@ -376,8 +403,23 @@ __global__ __launch_bounds__(256) void cached_prep_kernel(cached::Args A, cached
     }
   }
   if (is_q) {
+    const int64_t at = (int64_t)n * A.nh + r;
+    if constexpr (F8) {  // fp16, the row's largest value between 2^14 and 2^15
+      float top = 0.f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) wk.q[((int64_t)n * A.nh + r) * HD + lane + 64 * e] = x[e];
+      for (int e = 0; e < E; ++e) top = fmaxf(top, kv::finite_abs(x[e]));
+      const int e0 = (int)(__float_as_uint(wave_max_fast(top)) >> 23) - 141, ex = e0 < -100 ? -100 : e0;  // (or below, or zeros)
+      const float inv = kv::pow2(-ex);
+      if (lane == 0) wk.scale[at] = kv::pow2(ex);
+#pragma unroll
+      for (int e = 0; e < E; ++e) wk.q[at * HD + lane + 64 * e] = __builtin_bit_cast(uint16_t, (_Float16)(x[e] * inv));
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        wk.q[(2 * at) * HD + lane + 64 * e] = (uint16_t)(__float_as_uint(x[e]) >> 16);
+        wk.q[(2 * at + 1) * HD + lane + 64 * e] = f2bf(copysignf(low<false>(fabsf(x[e])), x[e]));
+      }
+    }
     return;
   }
   const int64_t row = ((int64_t)n * A.nkv + j) * A.own.T;
@@ -410,11 +452,11 @@ __global__ __launch_bounds__(256) void cached_prep_kernel(cached::Args A, cached
 //      for token 16 g + 8 u + e: the lane's own scores are its operand.  O's lane (c, g) has row c, dims 16 x + 4 g + r, so
 //      the running maximum's corrections are a number per lane.
 template <int HD, bool F8, int RT>
-__device__ __forceinline__ void split(const cached::Args& A, const cached::Work& wk, const cached::Item& it, cached::SplitLds<HD, RT>& lds,
+__device__ __forceinline__ void split(const cached::Args& A, const cached::Work& wk, const cached::Item& it, cached::SplitLds<HD, F8, RT>& lds,
                                       float scale2) {
   using namespace cached;
-  typedef SplitLds<HD, RT> Lds;
-  constexpr int R = Lds::R, LQ = Lds::LQ, DS = Lds::DS;
+  typedef SplitLds<HD, F8, RT> Lds;
+  constexpr int PARTS = Lds::PARTS, R = Lds::R, LQ = Lds::LQ, DS = Lds::DS;
   constexpr int KS = HD / 32, X = HD / 16;  // 32-dim steps of the scores, 16-dim tiles of the output
   auto& qs = lds.qs;
   auto& so = lds.so;
@@ -477,23 +519,20 @@ __device__ __forceinline__ void split(const cached::Args& A, const cached::Work&
     load_v(b);
   }
   __builtin_amdgcn_sched_barrier(0);
-  // ---- q into LDS, as a high and a low bf16 part
-  for (int i = tid; i < R * (HD / 8); i += 64 * WAVES) {
-    const int q = i / (HD / 8), d = 8 * (i % (HD / 8));
-    f32x4 v[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-    if (rown[q] >= 0) {
-      const f32x4* p = reinterpret_cast<const f32x4*>(&wk.q[((int64_t)rown[q] * A.nh + rowh[q]) * HD + d]);
-      v[0] = p[0], v[1] = p[1];
-    }
-    u32x4 hi, lo;
+  // ---- q into LDS
+#pragma unroll 4
+  for (int i = tid; i < PARTS * R * (HD / 8); i += 64 * WAVES) {
+    const int q = i / (HD / 8) / PARTS, h = i / (HD / 8) % PARTS, d = 8 * (i % (HD / 8));
+    u32x4 v = {0, 0, 0, 0};
+    if (rown[q] >= 0) v = *reinterpret_cast<const u32x4*>(&wk.q[(((int64_t)rown[q] * A.nh + rowh[q]) * PARTS + h) * HD + d]);
+    *reinterpret_cast<u32x4*>(&qs[h][q * LQ + d]) = v;
+  }
+  float sc[RT];  // row c's scores in powers of two
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float a = v[e / 2][2 * (e % 2)], b2 = v[e / 2][2 * (e % 2) + 1];
-      hi[e] = high2(a, b2);
-      lo[e] = f2bf2(copysignf(low<F8>(fabsf(a)), a), copysignf(low<F8>(fabsf(b2)), b2));
-    }
-    *reinterpret_cast<u32x4*>(&qs[0][q * LQ + d]) = hi;
-    *reinterpret_cast<u32x4*>(&qs[1][q * LQ + d]) = lo;
+  for (int t = 0; t < RT; ++t) {
+    const int q = 16 * t + c;
+    sc[t] = scale2;
+    if (F8 && rown[q] >= 0) sc[t] *= wk.scale[(int64_t)rown[q] * A.nh + rowh[q]];
   }
   lds_barrier();
   for (; b < b1; b += WAVES) {
@@ -508,20 +547,20 @@ __device__ __forceinline__ void split(const cached::Args& A, const cached::Work&
     // widened among this one's products; with 16, two waves a SIMD fill each other's gaps, and 256 registers are all there
     // are: two tiles at a time (6 registers too many, in scratch: 158 -> 186 us for 16 slots of 16384 to 32768 tokens).
     constexpr int AHEAD = RT == 2 && F8 ? 1 : 0, W = AHEAD ? 4 : 2;
-    u32x4 a[AHEAD + 1][W], q[AHEAD + 1][RT][2];
+    u32x4 a[AHEAD + 1][W], q[AHEAD + 1][RT][PARTS];
     auto query = [&](int s) {
       const int d = F8 ? 16 * (4 * (s / 2) + g) + 8 * (s % 2) : 8 * (4 * s + g);
 #pragma unroll
       for (int t = 0; t < RT; ++t)
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < PARTS; ++h)
           q[s % (AHEAD + 1)][t][h] = *reinterpret_cast<const u32x4*>(&qs[h][(16 * t + c) * LQ + d]);
     };
     auto keys = [&](int s, int i0) {
 #pragma unroll
       for (int i = 0; i < W; ++i) {
         const u32x4& k = kr[F8 ? s / 2 * 4 + i0 + i : s * 4 + i0 + i];
-        a[s % (AHEAD + 1)][i] = F8 ? widen(k[s % 2 * 2], k[s % 2 * 2 + 1]) : k;
+        a[s % (AHEAD + 1)][i] = F8 ? widen16(k[s % 2 * 2], k[s % 2 * 2 + 1]) : k;
       }
     };
     if (AHEAD) query(0), keys(0, 0);
@@ -533,13 +572,15 @@ __device__ __forceinline__ void split(const cached::Args& A, const cached::Work&
       for (int i0 = 0; i0 < 4; i0 += W) {
         if (!AHEAD) keys(s, i0);
 #pragma unroll
-        for (int h = 1; h >= 0; --h)
+        for (int h = PARTS - 1; h >= 0; --h)
 #pragma unroll
           for (int i = 0; i < W; ++i)
 #pragma unroll
-            for (int t = 0; t < RT; ++t)
-              D[t][i0 + i] = mma(a[s % (AHEAD + 1)][i], q[s % (AHEAD + 1)][t][h], D[t][i0 + i]);
-        if (AHEAD) mix<16>();
+            for (int t = 0; t < RT; ++t) {
+              const u32x4 &x = a[s % (AHEAD + 1)][i], &y = q[s % (AHEAD + 1)][t][h];
+              D[t][i0 + i] = F8 ? mma16(x, y, D[t][i0 + i]) : mma(x, y, D[t][i0 + i]);
+            }
+        if (AHEAD) mix<8>();
         __builtin_amdgcn_sched_barrier(0);
       }
     }
@@ -550,13 +591,14 @@ __device__ __forceinline__ void split(const cached::Args& A, const cached::Work&
     __builtin_amdgcn_sched_barrier(0);
     const int left = tokens - b * BT < BT ? tokens - b * BT : BT;  // tokens of this block in range
     // ---- softmax of row c over the lane's 16 tokens and the other g's
+    if constexpr (F8) {  // K's scales
 #pragma unroll
-    for (int t = 0; t < RT; ++t)
+      for (int t = 0; t < RT; ++t)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          D[t][i][r] *= F8 ? scale2 * __uint_as_float((kx1[i] >> (8 * r) & 0xffu) << 23) : scale2;
+          for (int r = 0; r < 4; ++r) D[t][i][r] *= __uint_as_float((kx1[i] >> (8 * r) & 0xffu) << 23);
+    }
     if (left < BT) {  // the last block: what lies behind the last token may be anything, and 0 times an infinity is NaN
       int k = left - 16 * g;  // this lane's tokens in range
 #pragma unroll
@@ -576,13 +618,15 @@ __device__ __forceinline__ void split(const cached::Args& A, const cached::Work&
     u32x4 pr[RT][2][2];  // [high and low part][step]
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
-      float mx = m[t];
+      float mx = -INFINITY;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r) mx = fmaxf(mx, D[t][i][r]);
       mx = fmaxf(mx, __shfl_xor(mx, 16, kWave));
       mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
+      const float to2 = F8 ? sc[t] : scale2;
+      mx = fmaxf(m[t], mx * to2);
       const float m0 = mx == -INFINITY ? 0.f : mx;
       const float fix = __builtin_amdgcn_exp2f(m[t] - m0);
       m[t] = mx;
@@ -593,7 +637,7 @@ __device__ __forceinline__ void split(const cached::Args& A, const cached::Work&
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int r = 0; r < 4; r += 2) {
-          float p0 = __builtin_amdgcn_exp2f(D[t][i][r] - m0), p1 = __builtin_amdgcn_exp2f(D[t][i][r + 1] - m0);
+          float p0 = __builtin_amdgcn_exp2f(fmaf(D[t][i][r], to2, -m0)), p1 = __builtin_amdgcn_exp2f(fmaf(D[t][i][r + 1], to2, -m0));
           l[t] += p0 + p1;
           if constexpr (F8) {  // V's scales
             p0 *= __uint_as_float((vx[i] >> (8 * r) & 0xffu) << 23);
@@ -693,7 +737,7 @@ __device__ __forceinline__ void split(const cached::Args& A, const cached::Work&
 template <int HD, bool F8, bool kPre>
 __global__ __launch_bounds__(256, !kPre && (HD < 256 || F8) ? 2 : 1) void cached_split_kernel(cached::Args A, cached::Work wk, float scale2) {
   using namespace cached;
-  __shared__ alignas(16) char raw[kPre ? sizeof(SplitLds<HD, 2>) : sizeof(SplitLds<HD, 1>)];
+  __shared__ alignas(16) char raw[kPre ? sizeof(SplitLds<HD, F8, 2>) : sizeof(SplitLds<HD, F8, 1>)];
   Item it = wk.items[blockIdx.x];
   it.tile = __builtin_amdgcn_readfirstlane(it.tile);
   it.row = __builtin_amdgcn_readfirstlane(it.row);
@@ -703,8 +747,8 @@ __global__ __launch_bounds__(256, !kPre && (HD < 256 || F8) ? 2 : 1) void cached
   it.tokens = __builtin_amdgcn_readfirstlane(it.tokens);
   it.part = __builtin_amdgcn_readfirstlane(it.part);
   if (it.b0 >= it.b1) return;
-  if (kPre && it.tile >= 0) split<HD, F8, 2>(A, wk, it, *reinterpret_cast<SplitLds<HD, 2>*>(raw), scale2);
-  else split<HD, F8, 1>(A, wk, it, *reinterpret_cast<SplitLds<HD, 1>*>(raw), scale2);
+  if (kPre && it.tile >= 0) split<HD, F8, 2>(A, wk, it, *reinterpret_cast<SplitLds<HD, F8, 2>*>(raw), scale2);
+  else split<HD, F8, 1>(A, wk, it, *reinterpret_cast<SplitLds<HD, F8, 1>*>(raw), scale2);
 }
 
 // grid (N * nh), 256 threads: HD / 4 lanes of 4 dims times groups of partials; the groups meet in LDS.

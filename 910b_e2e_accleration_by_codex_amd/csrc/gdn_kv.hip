@@ -2,7 +2,10 @@
 // written) and back.  Layout and quantisation: gdn_kv.h.
 //
 // Both are copies: bound by HBM, each value read once and written once.  One workgroup per (64-token cache block,
-// kv head, K or V).
+// kv head, K or V): a block is what lies together in the cache.  K's 16-byte pieces are one token's and go out as they are;
+// V's lie along the tokens and turn in LDS.  16 prompts of 200 to 1500 tokens (13.6 thousand, 4 heads of 256, bf16 to e4m3
+// and back, 84 MB each way): store 19.7 us (4.2 TB/s), load 17.9 us (4.7 TB/s), where a large copy runs at 4.97 TB/s; 517
+// tokens stored (3.2 MB) and 1541 loaded (9.5 MB): 7.5 and 6.6 us, a launch and a block's latency.
 #include "gdn_internal.h"
 #include "gdn_kv.h"
 

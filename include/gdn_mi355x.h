@@ -495,8 +495,11 @@ int gdn_kv_load(const void* k_cache, const void* v_cache, const uint8_t* k_exp, 
  *   gives a zero output; one inside the prefix writes nothing and attends to the prefix alone; one behind the cache
  *   row's end is not written and attends to all of the row.
  *   work: gdn_attn_cached_workspace_bytes(N, nh, nkv, hd, T, P, Tp) bytes, 256-byte aligned (-1: bad sizes).
- * hd in {64, 128, 256}; nh / nkv <= 16.  The query is rounded to bf16 once; scores, softmax and sums are fp32 (the
- * probabilities enter P V as bf16); the rotary angle is formed in double.  Replaces CBEngine._attn's decode attention
+ * hd in {64, 128, 256}; nh / nkv <= 16; N and P at most 1024.  Scores, softmax and sums are fp32; the query enters
+ * as fp16 in units of its row's largest value (bf16 caches: as two bf16 parts), the probabilities as two bf16 parts, the
+ * output is rounded once; the rotary angle is formed in double.  A graph that captured a call replays it for whatever pos, prefix_len and prefix_of hold then.  Calls that may
+ * overlap need a workspace each; its contents need no clearing, and one for more slots, tokens or prefixes holds fewer.
+ * Replaces CBEngine._attn's decode attention
  * (src/cb_engine.py:265-276) on a cache of half the bytes.
  */
 int64_t gdn_attn_cached_workspace_bytes(int N, int nh, int nkv, int hd, int64_t T, int P, int64_t Tp);
@@ -514,10 +517,13 @@ int gdn_attn_cached(const void* proj, int64_t proj_stride, const float* part, in
  * with w_i >= min_p (the largest always); the token is the first index at which the kept weights' running sum exceeds
  * u * their whole sum.  temperature <= 0 (or NaN): the first index of the maximum.  Logits of -inf or NaN are never
  * taken; a row that has nothing else gives -1.
+ * At most 8388608 logits a row (GDN_EUNSUP) and 65535 rows.  top_p's mass to reach is formed in double; top_p <= 0 is the
+ * largest alone.
  *   u [N] fp32 (or fp64 with u_is_f64) in [0, 1) on the device (values outside are cut to it).
  *   temperature, top_k, top_p, min_p: per row [N] on the device (fp32, int32, fp32, fp32), or NULL and the value *1 for
  *     every row.  out [N] int64.
- *   work: gdn_sample_workspace_bytes(N, V) bytes, 256-byte aligned; its contents need no clearing.
+ *   work: gdn_sample_workspace_bytes(N, V) bytes, 256-byte aligned; its contents need no clearing, one for more rows or
+ *     logits holds fewer, and calls that may overlap need one each.
  * Weights and sums are 64-bit, and sums do not depend on an order: the same inputs give the same token.  Replaces the
  * argmax over the engine's logits (src/cb_engine.py:170-172).
  */

@@ -299,6 +299,25 @@ def test_many_slots_and_prefixes(gdn, dev, N, P):
     check_cache(c, x, k, v, raw, (pos - full).tolist(), T)
 
 
+@pytest.mark.parametrize("fp8", [True, False])
+@pytest.mark.parametrize("scale", [0.0, 2.0 ** -60, 30.0])
+def test_queries_of_any_size(gdn, dev, fp8, scale):
+    """A query of zeros attends to all tokens alike; tiny ones nearly so; rows between the slots differ by many powers of
+    two (the query's norm weights are -1 + scale; half of the slots' rows are scaled below the norm's eps)."""
+    nh, kv, hd, T, N = 6, 1, 128, 192, 4
+    x = make(N, nh, kv, hd, T, fp8, 15)
+    x["qn"] = torch.full((hd,), scale - 1.0).to(BF) if scale in (0.0, 30.0) else x["qn"]
+    if scale == 30.0:  # scores of a few units all the same
+        x["proj"][:, :2 * nh * hd] *= 2.0 ** -18
+    if 0 < scale < 1:
+        x["proj"][::2, :2 * nh * hd] *= scale
+    pos = [0, 70, 128, 191]
+    out, _ = run(gdn, dev, x, pos, nh)
+    ref, _, _, _ = reference(x, pos, nh, fp8)
+    for n in range(N):
+        assert rel_l2(out[n], ref[n]) <= TOL, pos[n]
+
+
 def test_one_projection_for_all_slots_and_no_slots(gdn, dev):
     nh, kv, hd, T, N = 4, 2, 64, 64, 5
     x = make(N, nh, kv, hd, T, False, 14)
