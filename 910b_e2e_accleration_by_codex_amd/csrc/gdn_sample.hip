@@ -12,7 +12,14 @@
 // digit is one value, so that pass only counts.  The last pass also sums each chunk's mass above the bin, and the draw
 // resolves the last digit, finds the chunk and walks it.
 // Weights are computed in double and summed in 64-bit fixed point within a chunk (2^-50 of the largest), so that sums do
-// not depend on an order, and the draw itself is exact integer arithmetic on weights rounded to 2^-sh of the largest.
+// not depend on an order, and the draw itself is exact integer arithmetic on weights rounded to 2^-50 of the largest (fewer
+// bits from 4097 logits a row on, so that a row's sum stays below 2^62).
+//
+// Measured (all filters on; the launches' medians in us: first pass, passes, last pass, draw):
+//    1 x 248320 bf16: 6.5, 9.6, 13.9, 9.6      16 x 248320 bf16: 10.6, 11.4, 16.2, 15.0
+//   64 x 151936 fp32: 16.1, 22.8, 17.2, 15.7, 9.6, 6.0, 18.1, 12.1 (39 MB: a read of it at 6.07 TB/s is 6.4)
+// A pass over few rows is a chain of latencies: the histograms' merge and the choice of a bin (4 to 5), the row's load, the
+// LDS counters.  Over many rows the vector instructions bind: 50 to 75 an element, 20 of them its weight in double.
 #include "gdn_device.h"
 #include "gdn_internal.h"
 
@@ -181,28 +188,37 @@ template <typename T, int E> struct Chunk {
   __device__ __forceinline__ float operator[](int e) const { return cleaned(as_float<T>(x[e])); }
 };
 
-// Sums over lane l and those above it (scans run from the highest bin down), and over the whole wave.
-template <typename T> __device__ __forceinline__ T scan_down(T x) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const T y = __shfl_down(x, o, kWave);
-    if ((int)(threadIdx.x & 63) + o < 64) x += y;
+// Sums over lane l and those below it, and over the whole wave, by DPP (6 cross-lane reads through LDS cost a scan ten times
+// as much).  kRows: the rows of 16 lanes that add; the others, and lanes that have no source, add 0.
+template <int kCtrl, int kRows, typename T> __device__ __forceinline__ T dpp_add(T x) {
+  static_assert(sizeof(T) == 4 || sizeof(T) == 8, "");
+  if constexpr (sizeof(T) == 4) {
+    return x + __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), kCtrl, kRows, 0xf, false));
+  } else {
+    const u64 b = __builtin_bit_cast(u64, x);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, kCtrl, kRows, 0xf, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(b >> 32), kCtrl, kRows, 0xf, false);
+    return x + __builtin_bit_cast(T, (u64)hi << 32 | lo);
   }
-  return x;
 }
 template <typename T> __device__ __forceinline__ T scan_up(T x) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const T y = __shfl_up(x, o, kWave);
-    if ((int)(threadIdx.x & 63) >= o) x += y;
+  x = dpp_add<0x111, 0xf>(x);  // row_shr 1, 2, 4, 8: within 16 lanes
+  x = dpp_add<0x112, 0xf>(x);
+  x = dpp_add<0x114, 0xf>(x);
+  x = dpp_add<0x118, 0xf>(x);
+  x = dpp_add<0x142, 0xa>(x);         // lane 15 into lanes 16 .. 31, lane 47 into 48 .. 63
+  return dpp_add<0x143, 0xc>(x);      // lane 31 into lanes 32 .. 63
+}
+template <typename T> __device__ __forceinline__ T last_lane(T x) {
+  if constexpr (sizeof(T) == 4) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
+  } else {
+    const u64 b = __builtin_bit_cast(u64, x);
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)b, 63), hi = __builtin_amdgcn_readlane((int)(b >> 32), 63);
+    return __builtin_bit_cast(T, (u64)hi << 32 | lo);
   }
-  return x;
 }
-template <typename T> __device__ __forceinline__ T wave_total(T x) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o, kWave);
-  return x;
-}
+template <typename T> __device__ __forceinline__ T wave_total(T x) { return last_lane(scan_up(x)); }
 
 // A workgroup's scratch for choosing bins (W waves).
 template <int W> struct Scratch {
@@ -219,14 +235,14 @@ template <int W> struct Scratch {
 template <int W>
 __device__ __forceinline__ void choose(const Hist& h, bool root, const Work& wk, const Row& r, const Weights& wt, int n, int S,
                                        int levels, Scratch<W>& sc, double base, double& w) {
-  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, bin = 4 * (63 - lane);  // this lane's 4 bins
   const int level = root ? 0 : sc.st.level;
   const bool values = level == levels - 1;  // a bin is one value: its mass is its count times its weight
   const bool weigh = r.by_p && !values;
   uint32_t c[4] = {0, 0, 0, 0};
   double m[4] = {0, 0, 0, 0};
-  const uint32_t* hc = h.count + (int64_t)n * S * BINS + 4 * lane;
-  const u64* hm = h.mass + (int64_t)n * S * BINS + 4 * lane;
+  const uint32_t* hc = h.count + (int64_t)n * S * BINS + bin;
+  const u64* hm = h.mass + (int64_t)n * S * BINS + bin;
   if (weigh) {
 #pragma unroll 2
     for (int s = wid; s < S; s += W) {
@@ -239,47 +255,47 @@ __device__ __forceinline__ void choose(const Hist& h, bool root, const Work& wk,
       m[2] = fma((double)m1.x, f, m[2]), m[3] = fma((double)m1.y, f, m[3]);
     }
   } else {
-#pragma unroll 2
+#pragma unroll 4
     for (int s = wid; s < S; s += W) {
       const uint4 c1 = *reinterpret_cast<const uint4*>(hc + (int64_t)s * BINS);
       c[0] += c1.x, c[1] += c1.y, c[2] += c1.z, c[3] += c1.w;
     }
   }
-  *reinterpret_cast<uint4*>(&sc.count[wid][4 * lane]) = uint4{c[0], c[1], c[2], c[3]};
-  *reinterpret_cast<double2*>(&sc.mass[wid][4 * lane]) = double2{m[0], m[1]};
-  *reinterpret_cast<double2*>(&sc.mass[wid][4 * lane + 2]) = double2{m[2], m[3]};
+  *reinterpret_cast<uint4*>(&sc.count[wid][bin]) = uint4{c[0], c[1], c[2], c[3]};
+  *reinterpret_cast<double2*>(&sc.mass[wid][bin]) = double2{m[0], m[1]};
+  *reinterpret_cast<double2*>(&sc.mass[wid][bin + 2]) = double2{m[2], m[3]};
   __syncthreads();
   if (wid == 0) {
     State st = sc.st;
 #pragma unroll
     for (int g = 1; g < W; ++g) {
-      const uint4 c1 = *reinterpret_cast<const uint4*>(&sc.count[g][4 * lane]);
+      const uint4 c1 = *reinterpret_cast<const uint4*>(&sc.count[g][bin]);
       c[0] += c1.x, c[1] += c1.y, c[2] += c1.z, c[3] += c1.w;
       if (weigh) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) m[e] += sc.mass[g][4 * lane + e];
+        for (int e = 0; e < 4; ++e) m[e] += sc.mass[g][bin + e];
       }
     }
     double v[4] = {0, 0, 0, 0};
     if (values) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        v[e] = wt(value_of(st.prefix << 8 | (uint32_t)(4 * lane + e), levels));
+        v[e] = wt(value_of(st.prefix << 8 | (uint32_t)(bin + e), levels));
         m[e] = c[e] ? (double)c[e] * v[e] : 0.0;
       }
     }
-    // running sums from the highest bin; cs[e], ms[e]: of the bins above bin 4 lane + e
+    // running sums from the highest bin; cs[e], ms[e]: of the bins above this lane's e-th
     uint32_t cs[4];
     double ms[4];
     cs[3] = 0, ms[3] = 0;
 #pragma unroll
     for (int e = 2; e >= 0; --e) cs[e] = cs[e + 1] + c[e + 1], ms[e] = ms[e + 1] + m[e + 1];
     const uint32_t csum = cs[0] + c[0];
-    const double msum = ms[0] + m[0], mscan = scan_down(msum);
-    const uint32_t cb = scan_down(csum) - csum;
-    double mb = __shfl_down(mscan, 1, kWave);
-    if (lane == 63) mb = 0;
-    const double total = __shfl(mscan, 0, kWave);
+    const double msum = ms[0] + m[0], mscan = scan_up(msum);
+    const uint32_t cb = scan_up(csum) - csum;
+    double mb = __shfl_up(mscan, 1, kWave);
+    if (lane == 0) mb = 0;
+    const double total = last_lane(mscan);
     if (root && st.kind == 2) st.target = r.p * (base < 0 ? total : base);
     // the highest bin that reaches what is looked for
     int hit = -1;
@@ -301,12 +317,12 @@ __device__ __forceinline__ void choose(const Hist& h, bool root, const Work& wk,
           if (c[e]) hit = e;
         hits = __ballot(hit >= 0);
       }
-      if (hits) hits &= -hits;
+      if (hits) hits = 1ull << (63 - __builtin_clzll(hits));
     }
-    if (hits && lane == 63 - __builtin_clzll(hits)) {
+    if (hits && lane == __builtin_ctzll(hits)) {
       st.left -= (int)(hit == 0 ? cs[0] : hit == 1 ? cs[1] : hit == 2 ? cs[2] : cs[3]);
       st.above += hit == 0 ? ms[0] : hit == 1 ? ms[1] : hit == 2 ? ms[2] : ms[3];
-      st.prefix = st.prefix << 8 | (uint32_t)(4 * lane + hit);
+      st.prefix = st.prefix << 8 | (uint32_t)(bin + hit);
       ++st.level;
       sc.st = st;
       sc.bin_mass = hit == 0 ? m[0] : hit == 1 ? m[1] : hit == 2 ? m[2] : m[3];
@@ -623,8 +639,8 @@ __global__ __launch_bounds__(sample::DT) void sample_draw_kernel(sample::Job J, 
           found_before = upto - m;
           found_ties = before;
         }
-        sum = __shfl(upto, 63, kWave);
-        ties = __shfl(upto_t, 63, kWave);
+        sum = last_lane(upto);
+        ties = last_lane(upto_t);
       }
       u = u > 0.0 ? u < 1.0 ? u : 0x1.fffffffffffffp-1 : 0.0;
       const u64 U = (u64)(u * 0x1p53);
