@@ -16,9 +16,9 @@
 // bits from 4097 logits a row on, so that a row's sum stays below 2^62).
 //
 // Measured (all filters on; the launches' medians in us: first pass, passes, last pass, draw):
-//    1 x 248320 bf16: 6.5, 9.6, 13.9, 9.6      16 x 248320 bf16: 10.6, 11.4, 16.2, 15.0
-//   64 x 151936 fp32: 16.1, 22.8, 17.2, 15.7, 9.6, 6.0, 18.1, 12.1 (39 MB: a read of it at 6.07 TB/s is 6.4)
-// A pass over few rows is a chain of latencies: the histograms' merge and the choice of a bin (4 to 5), the row's load, the
+//    1 x 248320 bf16: 6.5, 8.6, 13.3, 7.4      16 x 248320 bf16: 10.4, 10.5, 15.1, 13.2
+//   64 x 151936 fp32: 15.5, 22.3, 16.1, 15.0, 9.6, 5.9, 18.0, 10.3 (39 MB: a read of it at 6.07 TB/s is 6.4)
+// A pass over few rows is a chain of latencies: the histograms' merge and the choice of a bin (3 to 4), the row's load, the
 // LDS counters.  Over many rows the vector instructions bind: 50 to 75 an element, 20 of them its weight in double.
 #include "gdn_device.h"
 #include "gdn_internal.h"
@@ -209,15 +209,16 @@ template <typename T> __device__ __forceinline__ T scan_up(T x) {
   x = dpp_add<0x142, 0xa>(x);         // lane 15 into lanes 16 .. 31, lane 47 into 48 .. 63
   return dpp_add<0x143, 0xc>(x);      // lane 31 into lanes 32 .. 63
 }
-template <typename T> __device__ __forceinline__ T last_lane(T x) {
+template <typename T> __device__ __forceinline__ T of_lane(T x, int l) {  // l uniform
   if constexpr (sizeof(T) == 4) {
-    return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
+    return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), l));
   } else {
     const u64 b = __builtin_bit_cast(u64, x);
-    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)b, 63), hi = __builtin_amdgcn_readlane((int)(b >> 32), 63);
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)b, l), hi = __builtin_amdgcn_readlane((int)(b >> 32), l);
     return __builtin_bit_cast(T, (u64)hi << 32 | lo);
   }
 }
+template <typename T> __device__ __forceinline__ T last_lane(T x) { return of_lane(x, 63); }
 template <typename T> __device__ __forceinline__ T wave_total(T x) { return last_lane(scan_up(x)); }
 
 // A workgroup's scratch for choosing bins (W waves).
@@ -230,12 +231,13 @@ template <int W> struct Scratch {
   uint32_t bin_count;
 };
 // One digit: the row's chunks merged, and by the first wave the bin in which the cut lies (sc.st).  root: the descent's
-// first digit, whose masses are relative to the chunks' own maxima (top_p: of mass, its target's base; below 0: the row's
-// whole mass).  The caller has a barrier in front.
+// first digit, whose masses are relative to the chunks' own maxima (first: the weights of the first 64 of these, a lane
+// each), with top_p's target p times `base` (below 0: times the row's whole mass).  Before anything but the first descent's
+// root the caller has a barrier.
 template <int W>
 __device__ __forceinline__ void choose(const Hist& h, bool root, const Work& wk, const Row& r, const Weights& wt, int n, int S,
-                                       int levels, Scratch<W>& sc, double base, double& w) {
-  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, bin = 4 * (63 - lane);  // this lane's 4 bins
+                                       int levels, Scratch<W>& sc, double first, double base, double& w) {
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), bin = 4 * (63 - lane);  // this lane's 4 bins
   const int level = root ? 0 : sc.st.level;
   const bool values = level == levels - 1;  // a bin is one value: its mass is its count times its weight
   const bool weigh = r.by_p && !values;
@@ -244,15 +246,26 @@ __device__ __forceinline__ void choose(const Hist& h, bool root, const Work& wk,
   const uint32_t* hc = h.count + (int64_t)n * S * BINS + bin;
   const u64* hm = h.mass + (int64_t)n * S * BINS + bin;
   if (weigh) {
-#pragma unroll 2
-    for (int s = wid; s < S; s += W) {
-      const uint4 c1 = *reinterpret_cast<const uint4*>(hc + (int64_t)s * BINS);
-      const ulonglong2 m0 = *reinterpret_cast<const ulonglong2*>(hm + (int64_t)s * BINS);
-      const ulonglong2 m1 = *reinterpret_cast<const ulonglong2*>(hm + (int64_t)s * BINS + 2);
-      const double f = root ? wt(wk.lmax[(int64_t)n * S + s]) * 0x1p-50 : 0x1p-50;
-      c[0] += c1.x, c[1] += c1.y, c[2] += c1.z, c[3] += c1.w;
-      m[0] = fma((double)m0.x, f, m[0]), m[1] = fma((double)m0.y, f, m[1]);
-      m[2] = fma((double)m1.x, f, m[2]), m[3] = fma((double)m1.y, f, m[3]);
+    constexpr int U = 2;  // chunks at a time, their loads ahead of their sums
+    for (int s0 = wid; s0 < S; s0 += U * W) {
+      uint4 c1[U];
+      ulonglong2 m0[U], m1[U];
+#pragma unroll
+      for (int x = 0; x < U; ++x) {
+        const int64_t s = s0 + x * W < S ? s0 + x * W : s0;
+        c1[x] = *reinterpret_cast<const uint4*>(hc + s * BINS);
+        m0[x] = *reinterpret_cast<const ulonglong2*>(hm + s * BINS);
+        m1[x] = *reinterpret_cast<const ulonglong2*>(hm + s * BINS + 2);
+      }
+#pragma unroll
+      for (int x = 0; x < U; ++x) {
+        const int s = s0 + x * W;
+        if (s >= S) break;
+        const double f = !root ? 0x1p-50 : (s < 64 ? of_lane(first, s) : wt(wk.lmax[(int64_t)n * S + s])) * 0x1p-50;
+        c[0] += c1[x].x, c[1] += c1[x].y, c[2] += c1[x].z, c[3] += c1[x].w;
+        m[0] = fma((double)m0[x].x, f, m[0]), m[1] = fma((double)m0[x].y, f, m[1]);
+        m[2] = fma((double)m1[x].x, f, m[2]), m[3] = fma((double)m1[x].y, f, m[3]);
+      }
     }
   } else {
 #pragma unroll 4
@@ -339,18 +352,24 @@ __device__ __forceinline__ void choose(const Hist& h, bool root, const Work& wk,
 template <int W>
 __device__ __forceinline__ void advance(const Job& J, const Work& wk, const Row& r, int n, int i, const double* table,
                                         Scratch<W>& sc) {
-  const bool root = i == 1;
-  if (!root) {
+  const int lane = threadIdx.x & 63;
+  const float mine = lane < J.S0 ? wk.lmax[(int64_t)n * J.S0 + lane] : -INFINITY;
+  float M;
+  if (i > 1) {
     // (a word a lane)
     const uint32_t* from = reinterpret_cast<const uint32_t*>(wk.state + (int64_t)((i - 1) & 1) * J.N + n);
     if (threadIdx.x < sizeof(State) / 4) reinterpret_cast<uint32_t*>(&sc.st)[threadIdx.x] = from[threadIdx.x];
-  } else if (threadIdx.x < 64) {
-    float m = -INFINITY;
-    for (int s = threadIdx.x; s < J.S0; s += 64) m = fmaxf(m, wk.lmax[(int64_t)n * J.S0 + s]);
-    m = wave_max_fast(m);
+    __syncthreads();
+    if (!sc.st.kind) return;
+    M = sc.st.M;
+  } else {  // every wave by itself: the histograms' loads need not wait for a barrier
+    M = mine;
+    for (int s = 64 + lane; s < J.S0; s += 64) M = fmaxf(M, wk.lmax[(int64_t)n * J.S0 + s]);
+    M = wave_max_fast(M);
+    const int kind = r.greedy || M == -INFINITY ? 0 : r.by_k ? 1 : r.by_p ? 2 : 0;
     if (threadIdx.x == 0) {
-      sc.st.M = m;
-      sc.st.kind = r.greedy || m == -INFINITY ? 0 : r.by_k ? 1 : r.by_p ? 2 : 0;
+      sc.st.M = M;
+      sc.st.kind = kind;
       sc.st.level = 0;
       sc.st.prefix = 0;
       sc.st.above = 0;
@@ -362,13 +381,15 @@ __device__ __forceinline__ void advance(const Job& J, const Work& wk, const Row&
       sc.st.cut_level = J.levels;
       sc.st.thr = 0;
     }
+    if (!kind) {
+      __syncthreads();
+      return;
+    }
   }
-  __syncthreads();
-  if (!sc.st.kind) return;
-  const Weights wt(r.t, sc.st.M, table);
+  const Weights wt(r.t, M, table);
   double base = -1.0, w;
   for (int h = i - 1;;) {
-    choose(wk.step[h], h == 0, wk, r, wt, n, h ? J.S : J.S0, J.levels, sc, base, w);
+    choose(wk.step[h], h == 0, wk, r, wt, n, h ? J.S : J.S0, J.levels, sc, h ? 0.0 : wt(mine), base, w);
     State st = sc.st;
     const bool full = st.level == J.levels;
     // a bin that is kept whole (all of it is wanted, or its only element) needs no further digits: the cut lies below it
@@ -508,7 +529,7 @@ __global__ __launch_bounds__(sample::TH, 4) void sample_pass_kernel(sample::Job 
   Chunk<T, EPT> c;
   c.load(row, at_turn(J, s, 0) + wid * WAVE, J.V);
   const Row r = row_of(J.par, n, J.V);
-  if (tid < 64) table[tid] = kPow[tid];
+  table[lane] = kPow[lane];  // (each wave, the same values: it may read them without a barrier)
   advance(J, wk, r, n, i, table, lds.sc);
   const State st = lds.sc.st;
   if (s == 0 && tid < (int)sizeof(State) / 4)
@@ -577,7 +598,7 @@ __global__ __launch_bounds__(sample::DT) void sample_draw_kernel(sample::Job J, 
   const Row r = row_of(J.par, n, J.V);
   const int was_kind = wk.state[(int64_t)((passes - 1) & 1) * J.N + n].kind;
   double u = J.u64_ ? J.u64_[n] : (double)J.u[n];
-  if (tid < 64) table[tid] = kPow[tid];
+  table[lane] = kPow[lane];  // (each wave, the same values: it may read them without a barrier)
   if (tid == 0) found = r.greedy ? INT32_MAX : -1;
   advance(J, wk, r, n, passes, table, sc);
   const State st = sc.st;
