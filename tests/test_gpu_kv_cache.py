@@ -180,6 +180,40 @@ def test_far_positions(gdn, dev):
     check(tail, expect(blank, x[0], x[1], [0], [0, 70], [58]))
 
 
+@pytest.mark.parametrize("dtype", [F8, BF])
+def test_graph_of_store_and_load(gdn, dev, dtype):
+    """Store and load captured with their batch on the device, replayed on other rows, lengths and starts (a batch that
+    ends before the packed tokens do: what lies behind is not written)."""
+    kv, hd, T, total = 2, 64, 256, 150
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    rows, cu, start = i32([0, 2]), i32([0, 70, 150]), i32([0, 10])
+    k, v = (torch.randn(total, kv, hd, generator=torch.Generator().manual_seed(i)).to(BF).to(dev) for i in range(2))
+    c, d = (gdn.KVCache.empty(3, kv, hd, T, dtype=dtype, device=dev) for _ in range(2))
+
+    def both():
+        gdn.kv_cache_store(c, k, v, rows, cu, start)
+        return gdn.kv_cache_load(c, rows, cu, start, total_tokens=total)
+    graph = gdn.GDNDecodeGraph(both, device=dev)
+    for t in (c.k, c.v, c.k_exp, c.v_exp):
+        if t is not None:
+            t.view(torch.uint8).fill_(127)
+    for t in (d.k, d.v, d.k_exp, d.v_exp):
+        if t is not None:
+            t.view(torch.uint8).fill_(127)
+    for r, n, s in (([0, 2], [70, 150], [0, 10]), ([1, 0], [1, 149], [255, 64]), ([2, 2], [33, 100], [100, 133])):
+        rows.copy_(i32(r))
+        cu.copy_(i32([0] + n))
+        start.copy_(i32(s))
+        k.copy_(torch.randn(k.shape, generator=torch.Generator().manual_seed(n[0])))
+        gk, gv = graph.replay()
+        torch.cuda.synchronize()
+        gdn.kv_cache_store(d, k[:n[1]], v[:n[1]], r, [0] + n, s)
+        for x, y in zip(c, d):
+            assert x is None or torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+        wk, wv = gdn.kv_cache_load(d, r, [0] + n, s)
+        assert torch.equal(gk[:n[1]], wk) and torch.equal(gv[:n[1]], wv)
+
+
 def test_refusals(gdn, dev):
     c = gdn.KVCache.empty(2, 2, 64, 128, device=dev)
     x = torch.zeros(10, 2, 64, dtype=BF, device=dev)

@@ -131,3 +131,40 @@ def test_chunked_prefill_round_trip(gdn, dev):
 def test_decoder_refuses_a_prefix_without_a_cache(gdn, dev):
     with pytest.raises(ValueError, match="cache_dtype"):
         hybrid().HybridDecoder(small(), 2, [3, 4], 4, dev, prefix_ctx=10)
+
+
+def test_calls_at_once_on_two_streams(gdn, dev):
+    """Attention and sampling on two streams at once, each with a workspace of its own, give what they give alone; a
+    workspace that has served other sizes gives the same."""
+    nh, kv, hd, N, V = 8, 2, 128, 12, 20000
+    width = (2 * nh + 2 * kv) * hd
+    g = torch.Generator().manual_seed(3)
+    side = []
+    for i in range(2):
+        c = gdn.KVCache.empty(N, kv, hd, 1024, device=dev)
+        k, v = (torch.randn(N * 1000, kv, hd, generator=g).to(torch.bfloat16).to(dev) for _ in range(2))
+        gdn.kv_cache_store(c, k, v, list(range(N)))
+        side.append(dict(c=c, proj=torch.randn(N, width, generator=g).to(torch.bfloat16).to(dev),
+                         pos=torch.randint(0, 1000, (N,), generator=g).to(dev), l=torch.randn(N, V, generator=g).to(dev),
+                         u=torch.rand(N, generator=g).to(dev), aw=gdn.cached_attn_workspace(c, nh),
+                         sw=gdn.sample_workspace(2 * N, V, dev)))
+    w = torch.zeros(hd, dtype=torch.bfloat16, device=dev)
+    inv = 1.0 / (10000.0 ** (torch.arange(0, 32, 2, device=dev).float() / 32))
+
+    def step(s, own=True):
+        kw, sw = (dict(work=s["aw"]), s["sw"]) if own else ({}, None)
+        return (gdn.cached_decode_attention(s["proj"], s["pos"], w, w, inv, s["c"], nh, 32, **kw),
+                gdn.sample_tokens(s["l"], s["u"], 0.8, 50, 0.9, work=sw))
+    want = [step(s, False) for s in side]
+    gdn.sample_tokens(side[0]["l"].repeat(2, 1), side[0]["u"].repeat(2), work=side[0]["sw"])
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(device=dev) for _ in side]
+    for _ in range(5):
+        got = []
+        for s, st in zip(side, streams):
+            with torch.cuda.stream(st):
+                got.append([step(s) for _ in range(3)])
+        torch.cuda.synchronize()
+        for i, x in enumerate(got):
+            for a, t in x:
+                assert torch.equal(a, want[i][0]) and torch.equal(t, want[i][1])
