@@ -22,11 +22,11 @@
 // Measured, 24 query and 4 kv heads of 256 (a large read runs at 6.07 TB/s, a large bf16 product at 1374 TFLOP/s), the
 // kernels' medians in us:
 //                                               bytes    prep  split  combine  split's rate
-//   16 slots of 512 to 4096 tokens, e4m3       76 MB     4.8   17.8    4.0     4.3 TB/s
-//   the same, bf16                            152 MB     4.4   27.7    4.2     5.5 TB/s
-//   16 slots of 16384 to 32768 tokens, e4m3   809 MB     6.2  156      6.1     5.2 TB/s
-//   16 slots behind 8192 shared tokens, e4m3   35 MB     7.0   19.4    4.7     177 TFLOP/s
-//   64 slots behind 2 x 16384, e4m3           108 MB     9.8   74      5.4     354 TFLOP/s
+//   16 slots of 512 to 4096 tokens, e4m3       76 MB     4.2   17.8    4.0     4.3 TB/s
+//   the same, bf16                            152 MB     4.2   27.7    4.2     5.5 TB/s
+//   16 slots of 16384 to 32768 tokens, e4m3   809 MB     5.6  156      6.1     5.2 TB/s
+//   16 slots behind 8192 shared tokens, e4m3   35 MB     5.8   19.4    4.7     177 TFLOP/s
+//   64 slots behind 2 x 16384, e4m3           108 MB     7.3   74      5.4     354 TFLOP/s
 // Slots' own tokens are bound by HBM, and where few, by the latency of a workgroup's start and merge (7 us of the 17.8).
 // A prefix's tiles are bound by the vector instructions around the products (codes widened, the softmax, probabilities
 // split and scaled) at one wave a SIMD.
@@ -178,12 +178,12 @@ __device__ __forceinline__ int64_t prefix_len(const Args& A, int r) {
   const int64_t n = A.plen[r];
   return n < 0 ? 0 : n > A.pre.T ? A.pre.T : n;
 }
-__device__ __forceinline__ Slot slot_of(const Args& A, int n) {
+template <typename Len> __device__ __forceinline__ Slot slot_of(const Args& A, int n, Len len) {  // len(r): prefix r's tokens
   Slot s;
   const int64_t p = A.pos[n];
   s.prefix = A.pof ? A.pof[n] : -1;
   if (s.prefix < 0 || s.prefix >= A.P || p < 0) s.prefix = -1;
-  int64_t at = p - (s.prefix >= 0 ? prefix_len(A, s.prefix) : 0);
+  int64_t at = p - (s.prefix >= 0 ? len(s.prefix) : 0);
   if (p < 0 || at < 0) at = -1;
   s.own = at < A.own.T ? at + 1 : A.own.T;
   s.at = at < A.own.T ? at : -1;
@@ -195,18 +195,13 @@ struct PlanLds {
   int tokens[MAXN], first[MAXN + 1];
   // a prefix's slots, tokens, first tile, place in order, first range of all its tiles
   int count[MAXP], len[MAXP], tile[MAXP + 1], order[MAXP + 1], part[MAXP + 1];
-  unsigned long long cost;
+  uint64_t cost[4];  // each wave's slots' and prefixes'
   int own, pre, wave[4];
 };
 // The sum of x over the threads before this one (256 threads; s.wave is free before and after).
 __device__ __forceinline__ int before(int x, PlanLds& s) {
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
-  int up = x;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(up, o, kWave);
-    if (lane >= o) up += y;
-  }
+  const int up = scan_up(x);
   if (lane == 63) s.wave[wid] = up;
   __syncthreads();
   int at = up - x;
@@ -230,15 +225,14 @@ __device__ __forceinline__ int entry_of(const int* first, int n, int f) {
 __device__ __forceinline__ void make_plan(const Args& A, const Work& wk, int planner, int planners, PlanLds& s) {
   const int tid = threadIdx.x, G = A.nh / A.nkv;
   const int i0 = planner * 256 + tid, step = planners * 256;  // of what is written
-  if (tid == 0) s.cost = 0;
   for (int r = tid; r < A.P; r += 256) {
     s.count[r] = 0;
     s.len[r] = (int)prefix_len(A, r);
   }
   __syncthreads();
-  unsigned long long cost = 0;
+  uint64_t cost = 0;
   for (int n = tid; n < A.N; n += 256) {
-    const Slot x = slot_of(A, n);
+    const Slot x = slot_of(A, n, [&](int r) { return (int64_t)s.len[r]; });
     s.tokens[n] = (int)x.own;
     s.prefix[n] = x.prefix;
     cost += blocks(x.own);
@@ -262,12 +256,13 @@ __device__ __forceinline__ void make_plan(const Args& A, const Work& wk, int pla
     }
     if (r0 < r1 && r1 == A.P) s.tile[A.P] = sum >> 16;
   }
-  if (cost) atomicAdd(&s.cost, cost);
+  cost = wave_total(cost);
+  if ((tid & 63) == 0) s.cost[tid >> 6] = cost;
   __syncthreads();
   if (tid == 0) {
     // a workgroup a CU; of slots' own tokens, which HBM bounds, 4 that even out where there are many blocks (16 slots of
     // 16384 to 32768 tokens: 199 us with one, 154 with four; 64 slots behind 16384 shared tokens: 105 us with four, 91)
-    unsigned long long each = (s.cost + WGS / A.nkv) / (WGS / A.nkv + 1);
+    uint64_t each = (s.cost[0] + s.cost[1] + s.cost[2] + s.cost[3] + WGS / A.nkv) / (WGS / A.nkv + 1);
     if (each > 1 << 28) each = 1 << 28;
     s.pre = (int)((each + 2 * WAVES - 1) / (2 * WAVES)) * WAVES;
     if (each >= 4 * LONG) each = (each + 3) / 4;
@@ -299,9 +294,9 @@ __device__ __forceinline__ void make_plan(const Args& A, const Work& wk, int pla
     if (r >= 0) {
       p.tile = s.tile[r];
 #pragma unroll 4
-      for (int m = 0; m < n; m += 4) {
+      for (int m = 0; m < A.N; m += 4) {  // (as far for every slot: the reads are the same, and go out together)
         const int4 x = *reinterpret_cast<const int4*>(&s.prefix[m]);
-        p.rank += (x.x == r) + (m + 1 < n && x.y == r) + (m + 2 < n && x.z == r) + (m + 3 < n && x.w == r);
+        p.rank += (m < n && x.x == r) + (m + 1 < n && x.y == r) + (m + 2 < n && x.z == r) + (m + 3 < n && x.w == r);
       }
       wk.order[s.order[r] + p.rank] = n;
     }
@@ -370,7 +365,7 @@ __global__ __launch_bounds__(256) void cached_prep_kernel(cached::Args A, cached
   const int n = (int)(w / per), r = (int)(w % per);
   const bool is_q = r < A.nh, is_v = r >= A.nh + A.nkv;
   const int j = is_q ? r : is_v ? r - A.nh - A.nkv : r - A.nh;
-  const Slot s = slot_of(A, n);
+  const Slot s = slot_of(A, n, [&](int p) { return prefix_len(A, p); });
   if (!is_q && s.at < 0) return;
   float x[E];
   A.proj.row<E>(x, n, is_q ? (int64_t)r * 2 * HD + lane : (int64_t)2 * A.nh * HD + (int64_t)(r - A.nh) * HD + lane);

@@ -188,39 +188,6 @@ template <typename T, int E> struct Chunk {
   __device__ __forceinline__ float operator[](int e) const { return cleaned(as_float<T>(x[e])); }
 };
 
-// Sums over lane l and those below it, and over the whole wave, by DPP (6 cross-lane reads through LDS cost a scan ten times
-// as much).  kRows: the rows of 16 lanes that add; the others, and lanes that have no source, add 0.
-template <int kCtrl, int kRows, typename T> __device__ __forceinline__ T dpp_add(T x) {
-  static_assert(sizeof(T) == 4 || sizeof(T) == 8, "");
-  if constexpr (sizeof(T) == 4) {
-    return x + __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), kCtrl, kRows, 0xf, false));
-  } else {
-    const u64 b = __builtin_bit_cast(u64, x);
-    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, kCtrl, kRows, 0xf, false);
-    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(b >> 32), kCtrl, kRows, 0xf, false);
-    return x + __builtin_bit_cast(T, (u64)hi << 32 | lo);
-  }
-}
-template <typename T> __device__ __forceinline__ T scan_up(T x) {
-  x = dpp_add<0x111, 0xf>(x);  // row_shr 1, 2, 4, 8: within 16 lanes
-  x = dpp_add<0x112, 0xf>(x);
-  x = dpp_add<0x114, 0xf>(x);
-  x = dpp_add<0x118, 0xf>(x);
-  x = dpp_add<0x142, 0xa>(x);         // lane 15 into lanes 16 .. 31, lane 47 into 48 .. 63
-  return dpp_add<0x143, 0xc>(x);      // lane 31 into lanes 32 .. 63
-}
-template <typename T> __device__ __forceinline__ T of_lane(T x, int l) {  // l uniform
-  if constexpr (sizeof(T) == 4) {
-    return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), l));
-  } else {
-    const u64 b = __builtin_bit_cast(u64, x);
-    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)b, l), hi = __builtin_amdgcn_readlane((int)(b >> 32), l);
-    return __builtin_bit_cast(T, (u64)hi << 32 | lo);
-  }
-}
-template <typename T> __device__ __forceinline__ T last_lane(T x) { return of_lane(x, 63); }
-template <typename T> __device__ __forceinline__ T wave_total(T x) { return last_lane(scan_up(x)); }
-
 // A workgroup's scratch for choosing bins (W waves).
 template <int W> struct Scratch {
   uint32_t count[W][BINS];  // each wave's share of the chunks
