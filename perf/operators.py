@@ -14,7 +14,6 @@ A cache keeps the 64 tokens of a block in the order in which the attention kerne
 In e4m3 each (token, kv head) row has one power-of-two scale 2^e, kept as the byte e + 127: e is the smallest integer
 with max |x| <= 448 * 2^e over the row's finite values (at least -126; 0 for a row of zeros).
 """
-import functools
 import math
 
 import numpy as np
@@ -29,7 +28,6 @@ CACHE = {"fp8": F8, "bf16": BF}
 DTYPES = {"bf16": BF, "fp16": torch.float16, "fp32": torch.float32}
 
 
-@functools.lru_cache(None)
 def _pkg():
     import importlib
     return importlib.import_module(PKG)
