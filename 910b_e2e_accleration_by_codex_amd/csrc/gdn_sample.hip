@@ -11,9 +11,11 @@
 // target is, so a row with both descends twice.  bf16 has 2 digits, fp16 3 (as fp32 values), fp32 4; a bin of the last
 // digit is one value, so that pass only counts.  The last pass also sums each chunk's mass above the bin, and the draw
 // resolves the last digit, finds the chunk and walks it.
-// Weights are computed in double and summed in 64-bit fixed point within a chunk (2^-50 of the largest), so that sums do
-// not depend on an order, and the draw itself is exact integer arithmetic on weights rounded to 2^-50 of the largest (fewer
-// bits from 4097 logits a row on, so that a row's sum stays below 2^62).
+// Weights (within 4e-10 of their value: 2^n times a double from a table times a series in fp32) are summed in 64-bit fixed
+// point within a workgroup, so that sums do not depend on an order: in units of 2^-50 of the largest, behind the first pass
+// of that times its turns (rounded up to a power of two), so that the 65536 weights of 1 of 8 turns are 2^63.  The draw
+// itself is exact integer arithmetic on weights rounded to 2^-50 of the largest (fewer bits from 4097 logits a row on, so
+// that a row's sum stays below 2^62).
 //
 // Measured (all filters on; the launches' medians in us: first pass, passes, last pass, draw):
 //    1 x 248320 bf16: 6.5, 8.6, 13.3, 7.4      16 x 248320 bf16: 10.4, 10.5, 15.1, 13.2
@@ -96,6 +98,7 @@ struct Job {
   // a row's chunks; turns of a workgroup in the passes behind the first, and workgroups a row has in them
   int N, V, S0, turns, S, levels;
   double one;  // the draw's weights: whole numbers of 1 / one
+  double unit, per;  // the masses of the passes behind the first: whole numbers of per = 1 / unit
 };
 
 // The first element of workgroup s's turn, in the passes behind the first.
@@ -199,11 +202,11 @@ template <int W> struct Scratch {
 };
 // One digit: the row's chunks merged, and by the first wave the bin in which the cut lies (sc.st).  root: the descent's
 // first digit, whose masses are relative to the chunks' own maxima (first: the weights of the first 64 of these, a lane
-// each), with top_p's target p times `base` (below 0: times the row's whole mass).  Before anything but the first descent's
-// root the caller has a barrier.
+// each), with top_p's target p times `base` (below 0: times the row's whole mass); the other digits' masses are whole
+// numbers of `per`.  Before anything but the first descent's root the caller has a barrier.
 template <int W>
 __device__ __forceinline__ void choose(const Hist& h, bool root, const Work& wk, const Row& r, const Weights& wt, int n, int S,
-                                       int levels, Scratch<W>& sc, double first, double base, double& w) {
+                                       int levels, Scratch<W>& sc, double first, double per, double base, double& w) {
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), bin = 4 * (63 - lane);  // this lane's 4 bins
   const int level = root ? 0 : sc.st.level;
   const bool values = level == levels - 1;  // a bin is one value: its mass is its count times its weight
@@ -228,7 +231,7 @@ __device__ __forceinline__ void choose(const Hist& h, bool root, const Work& wk,
       for (int x = 0; x < U; ++x) {
         const int s = s0 + x * W;
         if (s >= S) break;
-        const double f = !root ? 0x1p-50 : (s < 64 ? of_lane(first, s) : wt(wk.lmax[(int64_t)n * S + s])) * 0x1p-50;
+        const double f = !root ? per : (s < 64 ? of_lane(first, s) : wt(wk.lmax[(int64_t)n * S + s])) * 0x1p-50;
         c[0] += c1[x].x, c[1] += c1[x].y, c[2] += c1[x].z, c[3] += c1[x].w;
         m[0] = fma((double)m0[x].x, f, m[0]), m[1] = fma((double)m0[x].y, f, m[1]);
         m[2] = fma((double)m1[x].x, f, m[2]), m[3] = fma((double)m1[x].y, f, m[3]);
@@ -356,7 +359,7 @@ __device__ __forceinline__ void advance(const Job& J, const Work& wk, const Row&
   const Weights wt(r.t, M, table);
   double base = -1.0, w;
   for (int h = i - 1;;) {
-    choose(wk.step[h], h == 0, wk, r, wt, n, h ? J.S : J.S0, J.levels, sc, h ? 0.0 : wt(mine), base, w);
+    choose(wk.step[h], h == 0, wk, r, wt, n, h ? J.S : J.S0, J.levels, sc, h ? 0.0 : wt(mine), J.per, base, w);
     State st = sc.st;
     const bool full = st.level == J.levels;
     // a bin that is kept whole (all of it is wanted, or its only element) needs no further digits: the cut lies below it
@@ -531,7 +534,7 @@ __global__ __launch_bounds__(sample::TH, 4) void sample_pass_kernel(sample::Job 
         if (count) {
           const int b = (k >> dsh & 255u) * COLS + tid % COLS;
           atomicAdd(&lds.h.count[b], 1u);
-          if (weigh) atomicAdd(&lds.h.mass[b], fixed(wt(v), 0x1p50));
+          if (weigh) atomicAdd(&lds.h.mass[b], fixed(wt(v), J.unit));
         }
       }
     }
@@ -802,6 +805,9 @@ extern "C" int gdn_sample(const void* logits, int64_t stride, int dtype, const v
   J.levels = dtype == GDN_BF16 ? 2 : dtype == GDN_F16 ? 3 : 4;
   J.one = 0x1p50;  // V weights of at most `one` stay below 2^62
   while (J.one > 1.0 && J.one * V > 0x1p62) J.one *= 0.5;
+  J.unit = 0x1p50;  // J.turns * CHUNK weights of at most `unit` stay at or below 2^63
+  for (int t = 1; t < J.turns; t *= 2) J.unit *= 0.5;
+  J.per = 1.0 / J.unit;
   const bool by_k = top_k || (top_k1 > 0 && top_k1 < V), by_p = top_p || top_p1 < 1.0;
   const hipStream_t st = (hipStream_t)stream;
   switch (dtype) {

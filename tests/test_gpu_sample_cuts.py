@@ -1,0 +1,36 @@
+"""GPU tests of where sampling cuts: masses of many near-equal weights in batches of many rows, and a top_p that asks for all
+that top_k left, against the oracle's sort in extended precision."""
+import pytest
+import torch
+
+from oracle import serving_oracle as so
+
+pytestmark = pytest.mark.gpu
+
+
+def crowded(kind, N, V, dtype, seed):
+    """Rows whose weights crowd together: thousands of them near the largest."""
+    g = torch.Generator().manual_seed(seed)
+    if kind == "halves":  # the first half a little above the second
+        l = torch.full((N, V), 1.0)
+        l[:, :V // 2] = 1.0625
+    elif kind == "bulk":  # nine in ten equal, the others below them, a few above
+        l = torch.where(torch.rand(N, V, generator=g) < 0.9, 1.0, 0.75)
+        l[:, ::V // 7] = 1.5
+    elif kind == "narrow":  # distinct values within a hundredth
+        l = 4.5 + 0.02 * (torch.rand(N, V, generator=g) - 0.5)
+    else:
+        l = torch.full((N, V), -2.0)
+    return l.to(dtype), torch.rand(N, generator=g)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("kind,N,V", [("halves", 64, 248320), ("bulk", 64, 151936), ("narrow", 128, 248320), ("equal", 17, 248320),
+                                      ("bulk", 256, 50001), ("halves", 1100, 8193)])
+@pytest.mark.parametrize("par", [(1.0, 0, 0.3, 0.0), (1.0, 0, 0.5, 0.0), (0.7, 0, 0.9, 0.01), (1.0, 40000, 0.6, 0.0)])
+def test_many_rows_of_crowded_weights(gdn, dev, dtype, kind, N, V, par):
+    """A workgroup sums the weights of several chunks (2 to 8 of 8192 logits), and 65536 weights of 1 have to fit."""
+    l, u = crowded(kind, N, V, dtype, N)
+    got = gdn.sample_tokens(l.to(dev), u.to(dev), *par).cpu()
+    some = torch.arange(0, N, N // 8)
+    assert torch.equal(got[some], so.sample(l[some], u[some].numpy(), *par))
