@@ -362,9 +362,12 @@ __device__ __forceinline__ void advance(const Job& J, const Work& wk, const Row&
     choose(wk.step[h], h == 0, wk, r, wt, n, h ? J.S : J.S0, J.levels, sc, h ? 0.0 : wt(mine), J.per, base, w);
     State st = sc.st;
     const bool full = st.level == J.levels;
+    // below top_k's cut (its whole mass, summed in another order, was a unit in the last place short of the target): all that
+    // top_k left is kept, and its cut stands
+    const bool beyond = st.kind == 2 && st.level <= st.k_level && st.prefix < st.k_path >> 8 * (st.k_level - st.level);
     // a bin that is kept whole (all of it is wanted, or its only element) needs no further digits: the cut lies below it
     const bool whole = !full && st.prefix && (st.kind == 1 ? st.left == (int)sc.bin_count : h > 0 && sc.bin_count == 1);
-    if (!full && !whole) {
+    if (!full && !whole && !beyond) {
       if (st.level >= st.k_level || st.k_path >> 8 * (st.k_level - st.level) != st.prefix) return;
       h = st.level;  // top_p's descent along top_k's
       continue;
@@ -374,7 +377,9 @@ __device__ __forceinline__ void advance(const Job& J, const Work& wk, const Row&
       st.k_path = st.prefix;
       base = whole ? st.above + sc.bin_mass : st.above + (double)st.left * w;
     }
-    if (whole) {
+    if (beyond) {
+      st.level = st.cut_level;
+    } else if (whole) {
       st.thr = st.prefix - 1;
       st.quota = 0;
     } else if (st.kind == 1) {

@@ -34,3 +34,17 @@ def test_many_rows_of_crowded_weights(gdn, dev, dtype, kind, N, V, par):
     got = gdn.sample_tokens(l.to(dev), u.to(dev), *par).cpu()
     some = torch.arange(0, N, N // 8)
     assert torch.equal(got[some], so.sample(l[some], u[some].numpy(), *par))
+
+
+@pytest.mark.parametrize("dtype,V,T,N", [(torch.float32, 3000, 7.3, 65000), (torch.float16, 200, 7.3, 65000), (torch.bfloat16, 200, 7.3, 65000)])
+@pytest.mark.parametrize("short", [2.0 ** -53, 2.0 ** -52])
+def test_top_p_next_to_one_keeps_to_top_k(gdn, dev, dtype, V, T, N, short):
+    """A top_p of one less a rounding or two asks for all that top_k left: its mass, summed along two descents, may differ in
+    the last place, and still nothing below top_k's cut is taken.  Logits in descending order and the largest random number:
+    the token is the last one kept."""
+    g = torch.Generator(device=dev).manual_seed(V)
+    l = torch.randn(N, V, generator=g, device=dev).mul(3).to(dtype).float().sort(-1, descending=True).values.to(dtype)
+    k = torch.randint(1, V, (N,), generator=g, device=dev).int()
+    u = torch.full((N,), 1 - 2.0 ** -53, dtype=torch.float64, device=dev)
+    got = gdn.sample_tokens(l, u, T, k, 1 - short)
+    assert int((got >= k).sum()) == 0
