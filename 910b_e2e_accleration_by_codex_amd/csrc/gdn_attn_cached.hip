@@ -13,21 +13,21 @@
 //      head) or 32 (a tile of a prefix's slots).
 //   3. cached_combine_kernel: per (slot, head) the partials merged by their maxima, and the gate.
 // Rounding: K and V enter as the cache holds them (e4m3 codes are fp16 and bf16 values, their scales multiply scores and
-// probabilities in fp32).  The query against e4m3 keys is rounded to fp16 once, in units of its row's largest value, an
-// eighth of the output's rounding (with the two parts below 64 slots behind 16384 shared tokens take 81 us instead of 74).
-// The query against bf16 keys, and the probabilities, enter the bf16 products as a high and a low part, two products each:
+// probabilities in fp32).  The query and the probabilities enter the products as a high and a low part, two products each:
 // one rounding of each to bf16 would nearly double the error of the rounded output (0.0031 against 0.0017 relative).  The
-// output is rounded once, to bf16.
+// query's parts are fp16 against e4m3 keys, in units of its row's largest value (22 bits and more), bf16 against bf16 keys,
+// and the probabilities' bf16 (16 bits).  A query of 11 bits would do at scores of a few units, but its error grows with
+// them: at scores of 400 the output would be off by 2 to 4 %.  The output is rounded once, to bf16.
 //
 // Measured, 24 query and 4 kv heads of 256 (a large read runs at 6.07 TB/s, a large bf16 product at 1374 TFLOP/s), the
 // kernels' medians in us:
 //                                               bytes    prep  split  combine  split's rate
-//   16 slots of 512 to 4096 tokens, e4m3       76 MB     4.2   17.8    4.0     4.3 TB/s
+//   16 slots of 512 to 4096 tokens, e4m3       76 MB     4.2   18.4    3.9     4.1 TB/s
 //   the same, bf16                            152 MB     4.2   27.7    4.2     5.5 TB/s
-//   16 slots of 16384 to 32768 tokens, e4m3   809 MB     5.6  156      6.1     5.2 TB/s
-//   16 slots behind 8192 shared tokens, e4m3   35 MB     5.8   19.4    4.7     177 TFLOP/s
-//   64 slots behind 2 x 16384, e4m3           108 MB     7.3   74      5.4     354 TFLOP/s
-// Slots' own tokens are bound by HBM, and where few, by the latency of a workgroup's start and merge (7 us of the 17.8).
+//   16 slots of 16384 to 32768 tokens, e4m3   809 MB     5.9  158      6.3     5.1 TB/s
+//   16 slots behind 8192 shared tokens, e4m3   35 MB     6.0   21.0    4.8     164 TFLOP/s
+//   64 slots behind 2 x 16384, e4m3           108 MB     7.4   84      5.5     312 TFLOP/s
+// Slots' own tokens are bound by HBM, and where few, by the latency of a workgroup's start and merge (7 us of the 18.4).
 // A prefix's tiles are bound by the vector instructions around the products (codes widened, the softmax, probabilities
 // split and scaled) at one wave a SIMD.
 #include "gdn_attn.h"
@@ -123,8 +123,9 @@ struct TilePlan {
   int first, count;              // its partials
   int pad[2];
 };
-// workspace: q ([N, nh, hd] fp16 for an e4m3 cache, [N, nh, 2, hd] bf16 for a bf16 one), its rows' scales (fp32 [N, nh]) | partials: m, l (fp32 [parts, 2]) and o (fp32 [parts, hd]), parts = own_parts * nkv * G of
-// slots, then pre_parts * nkv * 32 of tiles | the plan
+// workspace: q's parts ([N, nh, 2, hd], fp16 for an e4m3 cache, bf16 for a bf16 one), its rows' scales (fp32 [N, nh]) |
+// partials: m, l (fp32 [parts, 2]) and o (fp32 [parts, hd]), parts = own_parts * nkv * G of slots, then
+// pre_parts * nkv * 32 of tiles | the plan
 struct Work {
   uint16_t* q;
   float *scale, *ml, *o;
@@ -333,11 +334,10 @@ __device__ __forceinline__ void make_plan(const Args& A, const Work& wk, int pla
     wk.items[item + i] = x;
   }
 }
-template <int HD, bool F8, int RT> struct SplitLds {
-  static constexpr int PARTS = F8 ? 1 : 2;        // of q
+template <int HD, int RT> struct SplitLds {
   static constexpr int R = 16 * RT, LQ = HD + 8;  // query rows, and their pitch
   static constexpr int DS = 64;                   // dims per round of the merge
-  alignas(16) uint16_t qs[PARTS][R * LQ];
+  alignas(16) uint16_t qs[2][R * LQ];  // q's high and low parts
   alignas(16) float so[WAVES][R][DS + 4];
   float sm[WAVES][R], sl[WAVES][R];
   int rown[R], rowh[R];  // each row's slot (-1: none) and head
@@ -407,7 +407,11 @@ __global__ __launch_bounds__(256) void cached_prep_kernel(cached::Args A, cached
       const float inv = kv::pow2(-ex);
       if (lane == 0) wk.scale[at] = kv::pow2(ex);
 #pragma unroll
-      for (int e = 0; e < E; ++e) wk.q[at * HD + lane + 64 * e] = __builtin_bit_cast(uint16_t, (_Float16)(x[e] * inv));
+      for (int e = 0; e < E; ++e) {
+        const _Float16 hi = (_Float16)(x[e] * inv), lo = (_Float16)(x[e] * inv - (float)hi);  // (not finite: hi alone)
+        wk.q[2 * at * HD + lane + 64 * e] = __builtin_bit_cast(uint16_t, hi);
+        wk.q[(2 * at + 1) * HD + lane + 64 * e] = fabsf(x[e]) < INFINITY ? __builtin_bit_cast(uint16_t, lo) : 0;
+      }
     } else {
 #pragma unroll
       for (int e = 0; e < E; ++e) {
@@ -447,11 +451,11 @@ __global__ __launch_bounds__(256) void cached_prep_kernel(cached::Args A, cached
 //      for token 16 g + 8 u + e: the lane's own scores are its operand.  O's lane (c, g) has row c, dims 16 x + 4 g + r, so
 //      the running maximum's corrections are a number per lane.
 template <int HD, bool F8, int RT>
-__device__ __forceinline__ void split(const cached::Args& A, const cached::Work& wk, const cached::Item& it, cached::SplitLds<HD, F8, RT>& lds,
+__device__ __forceinline__ void split(const cached::Args& A, const cached::Work& wk, const cached::Item& it, cached::SplitLds<HD, RT>& lds,
                                       float scale2) {
   using namespace cached;
-  typedef SplitLds<HD, F8, RT> Lds;
-  constexpr int PARTS = Lds::PARTS, R = Lds::R, LQ = Lds::LQ, DS = Lds::DS;
+  typedef SplitLds<HD, RT> Lds;
+  constexpr int R = Lds::R, LQ = Lds::LQ, DS = Lds::DS;
   constexpr int KS = HD / 32, X = HD / 16;  // 32-dim steps of the scores, 16-dim tiles of the output
   auto& qs = lds.qs;
   auto& so = lds.so;
@@ -516,10 +520,10 @@ __device__ __forceinline__ void split(const cached::Args& A, const cached::Work&
   __builtin_amdgcn_sched_barrier(0);
   // ---- q into LDS
 #pragma unroll 4
-  for (int i = tid; i < PARTS * R * (HD / 8); i += 64 * WAVES) {
-    const int q = i / (HD / 8) / PARTS, h = i / (HD / 8) % PARTS, d = 8 * (i % (HD / 8));
+  for (int i = tid; i < 2 * R * (HD / 8); i += 64 * WAVES) {
+    const int q = i / (HD / 8) / 2, h = i / (HD / 8) % 2, d = 8 * (i % (HD / 8));
     u32x4 v = {0, 0, 0, 0};
-    if (rown[q] >= 0) v = *reinterpret_cast<const u32x4*>(&wk.q[(((int64_t)rown[q] * A.nh + rowh[q]) * PARTS + h) * HD + d]);
+    if (rown[q] >= 0) v = *reinterpret_cast<const u32x4*>(&wk.q[(((int64_t)rown[q] * A.nh + rowh[q]) * 2 + h) * HD + d]);
     *reinterpret_cast<u32x4*>(&qs[h][q * LQ + d]) = v;
   }
   float sc[RT];  // row c's scores in powers of two
@@ -542,13 +546,13 @@ __device__ __forceinline__ void split(const cached::Args& A, const cached::Work&
     // widened among this one's products; with 16, two waves a SIMD fill each other's gaps, and 256 registers are all there
     // are: two tiles at a time (6 registers too many, in scratch: 158 -> 186 us for 16 slots of 16384 to 32768 tokens).
     constexpr int AHEAD = RT == 2 && F8 ? 1 : 0, W = AHEAD ? 4 : 2;
-    u32x4 a[AHEAD + 1][W], q[AHEAD + 1][RT][PARTS];
+    u32x4 a[AHEAD + 1][W], q[AHEAD + 1][RT][2];
     auto query = [&](int s) {
       const int d = F8 ? 16 * (4 * (s / 2) + g) + 8 * (s % 2) : 8 * (4 * s + g);
 #pragma unroll
       for (int t = 0; t < RT; ++t)
 #pragma unroll
-        for (int h = 0; h < PARTS; ++h)
+        for (int h = 0; h < 2; ++h)
           q[s % (AHEAD + 1)][t][h] = *reinterpret_cast<const u32x4*>(&qs[h][(16 * t + c) * LQ + d]);
     };
     auto keys = [&](int s, int i0) {
@@ -567,7 +571,7 @@ __device__ __forceinline__ void split(const cached::Args& A, const cached::Work&
       for (int i0 = 0; i0 < 4; i0 += W) {
         if (!AHEAD) keys(s, i0);
 #pragma unroll
-        for (int h = PARTS - 1; h >= 0; --h)
+        for (int h = 1; h >= 0; --h)
 #pragma unroll
           for (int i = 0; i < W; ++i)
 #pragma unroll
@@ -575,7 +579,7 @@ __device__ __forceinline__ void split(const cached::Args& A, const cached::Work&
               const u32x4 &x = a[s % (AHEAD + 1)][i], &y = q[s % (AHEAD + 1)][t][h];
               D[t][i0 + i] = F8 ? mma16(x, y, D[t][i0 + i]) : mma(x, y, D[t][i0 + i]);
             }
-        if (AHEAD) mix<8>();
+        if (AHEAD) mix<16>();
         __builtin_amdgcn_sched_barrier(0);
       }
     }
@@ -732,7 +736,7 @@ __device__ __forceinline__ void split(const cached::Args& A, const cached::Work&
 template <int HD, bool F8, bool kPre>
 __global__ __launch_bounds__(256, !kPre && (HD < 256 || F8) ? 2 : 1) void cached_split_kernel(cached::Args A, cached::Work wk, float scale2) {
   using namespace cached;
-  __shared__ alignas(16) char raw[kPre ? sizeof(SplitLds<HD, F8, 2>) : sizeof(SplitLds<HD, F8, 1>)];
+  __shared__ alignas(16) char raw[kPre ? sizeof(SplitLds<HD, 2>) : sizeof(SplitLds<HD, 1>)];
   Item it = wk.items[blockIdx.x];
   it.tile = __builtin_amdgcn_readfirstlane(it.tile);
   it.row = __builtin_amdgcn_readfirstlane(it.row);
@@ -742,8 +746,8 @@ __global__ __launch_bounds__(256, !kPre && (HD < 256 || F8) ? 2 : 1) void cached
   it.tokens = __builtin_amdgcn_readfirstlane(it.tokens);
   it.part = __builtin_amdgcn_readfirstlane(it.part);
   if (it.b0 >= it.b1) return;
-  if (kPre && it.tile >= 0) split<HD, F8, 2>(A, wk, it, *reinterpret_cast<SplitLds<HD, F8, 2>*>(raw), scale2);
-  else split<HD, F8, 1>(A, wk, it, *reinterpret_cast<SplitLds<HD, F8, 1>*>(raw), scale2);
+  if (kPre && it.tile >= 0) split<HD, F8, 2>(A, wk, it, *reinterpret_cast<SplitLds<HD, 2>*>(raw), scale2);
+  else split<HD, F8, 1>(A, wk, it, *reinterpret_cast<SplitLds<HD, 1>*>(raw), scale2);
 }
 
 // grid (N * nh), 256 threads: HD / 4 lanes of 4 dims times groups of partials; the groups meet in LDS.

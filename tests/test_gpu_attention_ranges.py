@@ -148,3 +148,42 @@ def test_a_million_shared_tokens(gdn, dev, fp8):
     ref = reference(x, pos, nh, c, prefix)
     for n in range(2):
         assert rel_l2(out[n], ref[n]) <= TOL, n
+
+
+@pytest.mark.parametrize("behind", [False, True])
+@pytest.mark.parametrize("fp8", [True, False])
+def test_large_scores(gdn, dev, fp8, behind):
+    """Scores of about 400 (a query norm weight of 128), and several tokens within one unit of each other at the top: a
+    query of 11 bits (2^-11 / sqrt(12) of a value in the mean square) has scores off by 0.015, and so the probabilities by more
+    than 1 %.  In two bf16 parts: 128 * 2^-17.7 = 0.0006."""
+    nh, kv, hd, T, N = 3, 3, 128, 8192, 4
+    x = inputs(N, nh, kv, hd, 21, qn=127.0)
+    c = cache_of(gdn, dev, N, kv, hd, T, fp8, 22)
+    if behind:  # the same history as a prefix for each slot
+        p = gdn.KVCache(*(None if y is None else y.clone() for y in c))
+        i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
+        prefix, c = gdn.SharedPrefix(p, i32([T] * N), i32(range(N))), gdn.KVCache.empty(N, kv, hd, 64, F8 if fp8 else BF, dev)
+        pos = [T] * N
+    else:
+        p, prefix, pos = c, None, [T - 1] * N
+    # of the highest 40 scores the largest group within one unit is made the top: what lies above it gets another token's key
+    for n in range(N):
+        k = values(p, "k", n, T)
+        qg = x["proj"][n].double()[:2 * nh * hd].view(nh, 2 * hd)
+        q = so.rms_rope(qg[:, :hd], x["qn"], pos[n], x["inv"], x["rd"], EPS).to(dev)
+        s = (q[:, None] * k).sum(-1) / math.sqrt(hd)
+        at = so.table(T, hd, "k", fp8).to(dev)
+        for h in range(kv):
+            low = int((s[h].abs()).argmin())
+            high = (s[h] > s[h].sort(descending=True).values[40]).nonzero()[:, 0]
+            order = high[s[h][high].argsort()]
+            top = max(range(len(order)), key=lambda i: int(((s[h][order] <= s[h][order[i]]) & (s[h][order] > s[h][order[i]] - 1)).sum()))
+            flat = (p.k.view(torch.uint8) if fp8 else p.k)[n, h].view(-1)
+            for t in order[top + 1:].tolist():
+                flat[at[t]] = flat[at[low]].clone()
+                if fp8:
+                    p.k_exp[n, h, t] = p.k_exp[n, h, low]
+    out = call(gdn, dev, x, pos, nh, c, prefix)
+    ref = reference(x, pos, nh, c, prefix)
+    for n in range(N):
+        assert rel_l2(out[n], ref[n]) <= TOL, n
