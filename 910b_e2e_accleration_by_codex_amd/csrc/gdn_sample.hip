@@ -38,8 +38,9 @@ constexpr int MOST = 1024 * CHUNK;  // logits of a row (the draw keeps its workg
 constexpr int TURNS = 8;          // at most
 typedef unsigned long long u64;
 
-struct Params {  // per row (device), or NULL and one value for all
-  const float *t, *p, *m;
+struct Params {  // per row (device; fp32, or fp64 where `f64` has the bit), or NULL and one value for all
+  const void *t, *p, *m;
+  int f64;
   const int32_t* k;
   double t1, p1, m1;
   int32_t k1;
@@ -49,11 +50,14 @@ struct Row {
   int32_t k;
   bool greedy, by_k, by_p;
 };
+__device__ __forceinline__ double param(const void* x, bool f64, int n) {
+  return f64 ? static_cast<const double*>(x)[n] : (double)static_cast<const float*>(x)[n];
+}
 __device__ __forceinline__ Row row_of(const Params& P, int n, int V) {
   Row r;
-  r.t = P.t ? (double)P.t[n] : P.t1;
-  r.p = P.p ? (double)P.p[n] : P.p1;
-  r.m = P.m ? (double)P.m[n] : P.m1;
+  r.t = P.t ? param(P.t, P.f64 & GDN_SAMPLE_F64_TEMPERATURE, n) : P.t1;
+  r.p = P.p ? param(P.p, P.f64 & GDN_SAMPLE_F64_TOP_P, n) : P.p1;
+  r.m = P.m ? param(P.m, P.f64 & GDN_SAMPLE_F64_MIN_P, n) : P.m1;
   r.k = P.k ? P.k[n] : P.k1;
   r.greedy = !(r.t > 0.0);  // NaN too
   if (r.p <= 0.0) r.p = 1e-300;  // the largest alone
@@ -778,8 +782,8 @@ extern "C" int64_t gdn_sample_workspace_bytes(int N, int V) {
   return sample_work(w, nullptr, J);
 }
 
-extern "C" int gdn_sample(const void* logits, int64_t stride, int dtype, const void* u, int u_is_f64, const float* temperature,
-                          const int32_t* top_k, const float* top_p, const float* min_p, double temperature1, int top_k1,
+extern "C" int gdn_sample(const void* logits, int64_t stride, int dtype, const void* u, int f64, const void* temperature,
+                          const int32_t* top_k, const void* top_p, const void* min_p, double temperature1, int top_k1,
                           double top_p1, double min_p1, int64_t* out, int N, int V, void* work, int64_t work_bytes,
                           void* stream) {
   clear_error();
@@ -790,7 +794,11 @@ extern "C" int gdn_sample(const void* logits, int64_t stride, int dtype, const v
   if (N == 0) return GDN_OK;
   GDN_REQUIRE(logits && u && out && work, "%s: null pointer", name);
   GDN_REQUIRE(N == 1 || stride >= V, "%s: row stride too small", name);
-  GDN_REQUIRE(aligned(logits, dtype == GDN_F32 ? 4 : 2) && aligned(work, 256) && aligned(out, 8) && aligned(u, u_is_f64 ? 8 : 4),
+  GDN_REQUIRE(f64 >= 0 && f64 < 16, "%s: bad fp64 flags", name);
+  const bool u_is_f64 = f64 & GDN_SAMPLE_F64_U;
+  GDN_REQUIRE(aligned(logits, dtype == GDN_F32 ? 4 : 2) && aligned(work, 256) && aligned(out, 8) && aligned(u, u_is_f64 ? 8 : 4) &&
+                  aligned(temperature, f64 & GDN_SAMPLE_F64_TEMPERATURE ? 8 : 4) && aligned(top_k, 4) &&
+                  aligned(top_p, f64 & GDN_SAMPLE_F64_TOP_P ? 8 : 4) && aligned(min_p, f64 & GDN_SAMPLE_F64_MIN_P ? 8 : 4),
               "%s: misaligned pointer (the workspace: 256 bytes)", name);
   GDN_REQUIRE(temperature || (temperature1 >= -1e300 && temperature1 <= 1e300), "%s: the temperature must be finite", name);
   GDN_REQUIRE((top_p || (top_p1 >= 0.0 && top_p1 <= 1.0)) && (min_p || (min_p1 >= 0.0 && min_p1 <= 1.0)),
@@ -806,7 +814,7 @@ extern "C" int gdn_sample(const void* logits, int64_t stride, int dtype, const v
   J.u = u_is_f64 ? nullptr : static_cast<const float*>(u);
   J.u64_ = u_is_f64 ? static_cast<const double*>(u) : nullptr;
   J.out = out;
-  J.par = {temperature, top_p, min_p, top_k, temperature1, top_p1, min_p1, top_k1};
+  J.par = {temperature, top_p, min_p, f64, top_k, temperature1, top_p1, min_p1, top_k1};
   J.levels = dtype == GDN_BF16 ? 2 : dtype == GDN_F16 ? 3 : 4;
   J.one = 0x1p50;  // V weights of at most `one` stay below 2^62
   while (J.one > 1.0 && J.one * V > 0x1p62) J.one *= 0.5;

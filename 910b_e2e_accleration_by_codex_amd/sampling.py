@@ -16,7 +16,7 @@ def sample_workspace(n_rows, vocab, device):
 
 
 def _param(what, x, N, dtype, device):
-    """(device pointer or None, value): a number for every row, or a tensor [N] on the device."""
+    """(device pointer or None, value, tensor kept alive): a number for every row, or a tensor [N] on the device."""
     if not isinstance(x, torch.Tensor):
         return None, x, None
     if dtype is torch.int32 and (x.dtype.is_floating_point or x.dtype is torch.bool):
@@ -25,14 +25,16 @@ def _param(what, x, N, dtype, device):
         raise ValueError(f"sample_tokens: {what} must be a number or a tensor of {N} entries on {device}")
     if x.dtype is torch.int64 and dtype is torch.int32:
         x = x.clamp(-1, 2 ** 31 - 1)
-    x = x.reshape(-1).to(dtype).contiguous()
+    if x.dtype is not torch.float64 or dtype is torch.int32:
+        x = x.to(dtype)
+    x = x.reshape(-1).contiguous()
     return x.data_ptr(), 0, x
 
 
 def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, work=None):
     """One token per row: int64 [N].  logits [N, V] bf16, fp16 or fp32 (a step's output; unit inner stride); u [N] fp32 or
-    fp64 in [0, 1), the rows' random numbers.  temperature, top_k, top_p, min_p: numbers, or tensors [N] on the device
-    (one per request).
+    fp64 in [0, 1), the rows' random numbers.  temperature, top_k, top_p, min_p: numbers (as doubles), or tensors [N] on
+    the device (one per request; fp64 ones as they are, others as fp32, top_k as int32).
 
     With w_i = exp((l_i - max l) / temperature): of the top_k largest logits (<= 0: all; ties go to the lowest index),
     of these the fewest most likely whose mass reaches top_p of their mass, of these those with w_i >= min_p, the
@@ -58,6 +60,7 @@ def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, wor
     k, k1, keep_k = _param("top_k", top_k, N, torch.int32, dev)
     p, p1, keep_p = _param("top_p", top_p, N, torch.float32, dev)
     m, m1, keep_m = _param("min_p", min_p, N, torch.float32, dev)
+    f64 = sum(bit for bit, x in ((1, u), (2, keep_t), (4, keep_p), (8, keep_m)) if x is not None and x.dtype is torch.float64)
     if logits.stride(1) != 1 or (N > 1 and logits.stride(0) < V):  # (one row for all, too)
         logits = logits.contiguous()
     u = u.contiguous()
@@ -69,6 +72,6 @@ def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, wor
     elif not work.is_cuda or work.device != dev or not work.is_contiguous():
         raise ValueError(f"sample_tokens: work must be a contiguous tensor on {dev}")
     _lib.call_on(logits, "gdn_sample", logits.data_ptr(), logits.stride(0) if N > 1 else V, code, u.data_ptr(),
-              int(u.dtype == torch.float64), t, k, p, m, float(t1), int(k1), float(p1), float(m1), out.data_ptr(), N, V,
+              f64, t, k, p, m, float(t1), int(k1), float(p1), float(m1), out.data_ptr(), N, V,
               work.data_ptr(), work.numel() * work.element_size(), _lib.stream_of(logits))
     return out

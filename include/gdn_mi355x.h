@@ -520,17 +520,19 @@ int gdn_attn_cached(const void* proj, int64_t proj_stride, const float* part, in
  * taken; a row that has nothing else gives -1.
  * At most 8388608 logits a row (GDN_EUNSUP) and 65535 rows.  top_p's mass to reach is formed in double; top_p <= 0 is the
  * largest alone.
- *   u [N] fp32 (or fp64 with u_is_f64) in [0, 1) on the device (values outside are cut to it).
+ *   u [N] fp32 in [0, 1) on the device (values outside are cut to it).
  *   temperature, top_k, top_p, min_p: per row [N] on the device (fp32, int32, fp32, fp32), or NULL and the value *1 for
- *     every row.  out [N] int64.
+ *     every row.  f64: a sum of GDN_SAMPLE_F64_*, for those of u, temperature, top_p and min_p that are fp64 instead.
+ *   out [N] int64.
  *   work: gdn_sample_workspace_bytes(N, V) bytes, 256-byte aligned; its contents need no clearing, one for more rows or
  *     logits holds fewer, and calls that may overlap need one each.
  * Weights and sums are 64-bit, and sums do not depend on an order: the same inputs give the same token.  Replaces the
  * argmax over the engine's logits (src/cb_engine.py:170-172).
  */
 int64_t gdn_sample_workspace_bytes(int N, int V);
-int gdn_sample(const void* logits, int64_t stride, int dtype, const void* u, int u_is_f64, const float* temperature,
-               const int32_t* top_k, const float* top_p, const float* min_p, double temperature1, int top_k1, double top_p1,
+enum { GDN_SAMPLE_F64_U = 1, GDN_SAMPLE_F64_TEMPERATURE = 2, GDN_SAMPLE_F64_TOP_P = 4, GDN_SAMPLE_F64_MIN_P = 8 };
+int gdn_sample(const void* logits, int64_t stride, int dtype, const void* u, int f64, const void* temperature,
+               const int32_t* top_k, const void* top_p, const void* min_p, double temperature1, int top_k1, double top_p1,
                double min_p1, int64_t* out, int N, int V, void* work, int64_t work_bytes, void* stream);
 
 #ifdef __cplusplus

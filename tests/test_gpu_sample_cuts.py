@@ -48,3 +48,23 @@ def test_top_p_next_to_one_keeps_to_top_k(gdn, dev, dtype, V, T, N, short):
     u = torch.full((N,), 1 - 2.0 ** -53, dtype=torch.float64, device=dev)
     got = gdn.sample_tokens(l, u, T, k, 1 - short)
     assert int((got >= k).sum()) == 0
+
+
+def test_parameters_in_fp64_are_not_rounded(gdn, dev):
+    """A number and an fp64 tensor of it cut alike; in fp32 the same figures cut elsewhere."""
+    top = torch.full((3,), 1 - 2.0 ** -53, dtype=torch.float64, device=dev)
+    one = lambda x, dtype=torch.float64: torch.full((3,), x, dtype=dtype, device=dev)  # noqa: E731
+    flat = torch.zeros(3, 10, device=dev)
+    for p, want in ((0.3, 2), (0.6, 5)):  # 0.3 as fp32 is 0.30000001: a fourth token
+        assert gdn.sample_tokens(flat, top, 1.0, 0, p).tolist() == [want] * 3
+        assert gdn.sample_tokens(flat, top, 1.0, 0, one(p)).tolist() == [want] * 3
+        assert gdn.sample_tokens(flat, top, 1.0, 0, one(p, torch.float32)).tolist() == [want + 1] * 3
+    l = torch.tensor([[0.0, -1.0]], device=dev).expand(3, -1)
+    m = 0.36787944  # exp(-1) is 0.3678794412; as fp32 0.3678794503
+    assert gdn.sample_tokens(l, top, 1.0, 0, 1.0, m).tolist() == [1] * 3
+    assert gdn.sample_tokens(l, top, 1.0, 0, 1.0, one(m)).tolist() == [1] * 3
+    assert gdn.sample_tokens(l, top, 1.0, 0, 1.0, one(m, torch.float32)).tolist() == [0] * 3
+    t, m = 1 + 1e-8, 0.367879443  # exp(-1 / t) is 0.3678794449; t as fp32 is 1
+    assert gdn.sample_tokens(l, top, t, 0, 1.0, m).tolist() == [1] * 3
+    assert gdn.sample_tokens(l, top, one(t), 0, 1.0, m).tolist() == [1] * 3
+    assert gdn.sample_tokens(l, top, one(t, torch.float32), 0, 1.0, m).tolist() == [0] * 3
