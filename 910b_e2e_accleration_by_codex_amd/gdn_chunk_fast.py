@@ -63,6 +63,7 @@ class Varlen:
         if len(cu) < 2 or cu[0] != 0 or cu[-1] != T or any(y < x for x, y in zip(cu, cu[1:])):
             raise ValueError(f"cu_seqlens must be non-decreasing from 0 to {T}, got {cu[:8]}...")
         self.T = T
+        self.host = cu
         self.nseq = len(cu) - 1
         s0 = [0]
         for x, y in zip(cu, cu[1:]):

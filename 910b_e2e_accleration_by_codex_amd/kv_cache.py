@@ -106,9 +106,9 @@ def _int32(name, what, x, n, device):
     return _to_device_int32(x.reshape(-1).to(torch.int64), device)
 
 
-def _batch(name, rows, cu_seqlens, start, total, n_rows, device):
-    """Device int32 (rows, cu_seqlens, start) of a batch; what comes from the host is checked here, what is on the device
-    is cut to the cache by the kernels."""
+def _batch(name, rows, cu_seqlens, start, total, n_rows, length, device):
+    """Device int32 (rows, cu_seqlens, start) of a batch for a cache of n_rows rows of `length` tokens; what comes from the
+    host is checked here, what is on the device is cut to the cache by the kernels."""
     if isinstance(rows, Rows):
         rows = rows.dev
     elif not (isinstance(rows, torch.Tensor) and rows.is_cuda):
@@ -118,8 +118,9 @@ def _batch(name, rows, cu_seqlens, start, total, n_rows, device):
         rows = host
     rows = _int32(name, "rows", rows, None, device)
     nseq = rows.numel()
+    cu = None  # where the lengths are known here
     if isinstance(cu_seqlens, Varlen):
-        cu_seqlens = cu_seqlens.cu
+        cu, cu_seqlens = cu_seqlens.host, cu_seqlens.cu
     elif cu_seqlens is not None and not (isinstance(cu_seqlens, torch.Tensor) and cu_seqlens.is_cuda):
         cu = [int(x) for x in (cu_seqlens.tolist() if isinstance(cu_seqlens, torch.Tensor) else cu_seqlens)]
         if len(cu) != nseq + 1 or cu[0] != 0 or cu[-1] != total or any(y < x for x, y in zip(cu, cu[1:])):
@@ -129,6 +130,15 @@ def _batch(name, rows, cu_seqlens, start, total, n_rows, device):
         cu_seqlens = _int32(name, "cu_seqlens", cu_seqlens, nseq + 1, device)
     elif nseq and total % nseq:
         raise ValueError(f"{name}: {total} tokens do not divide into {nseq} sequences of one length (give cu_seqlens)")
+    elif nseq:
+        cu = range(0, total + 1, total // nseq) if total else [0] * (nseq + 1)
+    if start is None or not (isinstance(start, torch.Tensor) and start.is_cuda):
+        first = [0] * nseq if start is None else start.reshape(-1).tolist() if isinstance(start, torch.Tensor) else list(start)
+        lens = [0] * nseq if cu is None else [y - x for x, y in zip(cu, cu[1:])]
+        for s, (t, n) in enumerate(zip(first, lens)):
+            if t < 0 or t + n > length:
+                raise ValueError(f"{name}: sequence {s} ({n} tokens from position start = {t}) does not lie in the cache's "
+                                 f"{length} positions")
     if start is not None:
         start = _int32(name, "start", start, nseq, device)
     return rows, cu_seqlens, start, nseq
@@ -147,8 +157,8 @@ def kv_cache_store(cache, k, v, rows, cu_seqlens=None, start=None):
     k, v [tokens, kv, hd] bf16, fp16 or fp32 (as a prefill leaves them: any token and head strides, so a transposed view
     of HF's [kv, tokens, hd] needs no copy).  Sequence s is the tokens cu_seqlens[s] .. cu_seqlens[s + 1] (None: equal
     lengths) and goes to positions start[s], start[s] + 1, .. (None: 0) of cache row rows[s].  rows, cu_seqlens and start:
-    int32 tensors on the device, or lists / CPU tensors (a Rows / Varlen where one is at hand).  Rows and positions outside the
-    cache are not written; no two sequences may write the same place."""
+    int32 tensors on the device, or lists / CPU tensors (a Rows / Varlen where one is at hand), which are
+    checked.  Of what is on the device, rows and positions outside the cache are not written; no two sequences may write the same place."""
     name = "kv_cache_store"
     code, R, kv, hd, T, index = _check(name, cache)
     _lib.require_cuda(k, v)
@@ -160,7 +170,7 @@ def kv_cache_store(cache, k, v, rows, cu_seqlens=None, start=None):
     if k.get_device() != index or v.get_device() != index:
         raise ValueError(f"{name}: k and v must be on the cache's device {dev}")
     total = k.shape[0]
-    rows, cu, start, nseq = _batch(name, rows, cu_seqlens, start, total, R, dev)
+    rows, cu, start, nseq = _batch(name, rows, cu_seqlens, start, total, R, T, dev)
     if total == 0 or nseq == 0:
         if total:
             raise ValueError(f"{name}: {total} tokens and no rows")
@@ -175,8 +185,8 @@ def kv_cache_store(cache, k, v, rows, cu_seqlens=None, start=None):
 def kv_cache_load(cache, rows, cu_seqlens, start=None, total_tokens=None):
     """The keys and values that a cache holds, as packed bf16 rows: sequence s gives positions start[s] .. start[s] +
     (cu_seqlens[s + 1] - cu_seqlens[s]) - 1 of row rows[s].  Arguments as kv_cache_store; with cu_seqlens on the device give
-    ``total_tokens`` (its last entry) too, or it is read back.  Returns (k, v) [total_tokens, kv, hd] bf16; positions and
-    rows outside the cache are zeros, and tokens that no sequence covers (behind the last one of a padded batch) hold anything."""
+    ``total_tokens`` (its last entry) too, or it is read back.  Returns (k, v) [total_tokens, kv, hd] bf16; rows and
+    positions outside the cache (those on the device) are zeros, and tokens that no sequence covers (behind the last one of a padded batch) hold anything."""
     name = "kv_cache_load"
     code, R, kv, hd, T, _ = _check(name, cache)
     dev = cache.k.device
@@ -187,7 +197,7 @@ def kv_cache_load(cache, rows, cu_seqlens, start=None, total_tokens=None):
     total = int(total_tokens)
     if total < 0:
         raise ValueError(f"{name}: total_tokens must not be negative")
-    rows, cu, start, nseq = _batch(name, rows, cu_seqlens, start, total, R, dev)
+    rows, cu, start, nseq = _batch(name, rows, cu_seqlens, start, total, R, T, dev)
     if total and not nseq:
         raise ValueError(f"{name}: {total} tokens and no rows")
     k, v = torch.empty(2, total, kv, hd, dtype=torch.bfloat16, device=dev).unbind(0)
