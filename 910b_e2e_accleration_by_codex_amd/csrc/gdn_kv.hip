@@ -198,18 +198,16 @@ __global__ __launch_bounds__(256) void kv_store_kernel(const T* __restrict__ xk,
 #pragma unroll
       for (int i = 0; i < 4; ++i) put(out + (int64_t)(d + i) * 64 + 16 * a, w[i], 16 * a);
     }
-    return;
-  }
-  // 16 bytes (8 tokens of one dim) at a time, in the order in which they lie in the cache
-  for (int o = tid; o < HD * BT * S / 16; o += 256) {
-    const int dg = o / (64 * S), rest = o % (64 * S);  // 16 dims, then [16 dims][4] (e4m3) or [2][16 dims][4] (bf16)
-    const int u = rest / 64, m = rest / 4 % 16, a = rest % 4, d = 16 * dg + m, t = 16 * a + 8 * u;
-    uint32_t w[4];
+  } else {  // 8 tokens of one dim at a time, in the order in which they lie in the cache: 16 dims, then [2][16 dims][4]
+    for (int o = tid; o < HD * 8; o += 256) {
+      const int u = o / 64 % 2, m = o / 4 % 16, a = o % 4, d = o / 128 * 16 + m, t = 16 * a + 8 * u;
+      uint32_t w[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      w[j] = *reinterpret_cast<const uint16_t*>(&tile[(t + 2 * j) * PITCH + 2 * d]) |
-             (uint32_t) * reinterpret_cast<const uint16_t*>(&tile[(t + 2 * j + 1) * PITCH + 2 * d]) << 16;
-    put(out + (int64_t)o * 16, w, t);
+      for (int j = 0; j < 4; ++j)
+        w[j] = *reinterpret_cast<const uint16_t*>(&tile[(t + 2 * j) * PITCH + 2 * d]) |
+               (uint32_t) * reinterpret_cast<const uint16_t*>(&tile[(t + 2 * j + 1) * PITCH + 2 * d]) << 16;
+      put(out + (int64_t)o * 16, w, t);
+    }
   }
 }
 
@@ -234,29 +232,28 @@ __global__ __launch_bounds__(256) void kv_load_kernel(const uint8_t* __restrict_
   const bool is_v = blockIdx.z;
   const int64_t row = (int64_t)q.row * nkv + head;
   const uint8_t* in = (is_v ? vc : kc) + (row * len + t0) * HD * S;
-  if (is_v && there && F8) {
-    for (int o = tid; o < HD; o += 256) {
-      const int a = o % 4, d = o / 4 * 4;
-      u32x4 w[4];
+  if (is_v && there) {
+    if constexpr (F8) {
+      for (int o = tid; o < HD; o += 256) {
+        const int a = o % 4, d = o / 4 * 4;
+        u32x4 w[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const u32x4*>(in + (int64_t)(d + i) * 64 + 16 * a);
+        for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const u32x4*>(in + (int64_t)(d + i) * 64 + 16 * a);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        uint32_t x[4] = {w[0][j], w[1][j], w[2][j], w[3][j]};
-        transpose4(x);
+        for (int j = 0; j < 4; ++j) {
+          uint32_t x[4] = {w[0][j], w[1][j], w[2][j], w[3][j]};
+          transpose4(x);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) *reinterpret_cast<uint32_t*>(&tile[(16 * a + 4 * j + i) * PITCH + d]) = x[i];
+          for (int i = 0; i < 4; ++i) *reinterpret_cast<uint32_t*>(&tile[(16 * a + 4 * j + i) * PITCH + d]) = x[i];
+        }
       }
-    }
-  } else if (is_v && there) {
-    for (int o = tid; o < HD * BT * S / 16; o += 256) {
-      const int dg = o / (64 * S), rest = o % (64 * S);
-      const int u = rest / 64, m = rest / 4 % 16, a = rest % 4, d = 16 * dg + m, t = 16 * a + 8 * u;
-      const u32x4 w = *reinterpret_cast<const u32x4*>(in + (int64_t)o * 16);
+    } else {
+      for (int o = tid; o < HD * 8; o += 256) {
+        const int u = o / 64 % 2, m = o / 4 % 16, a = o % 4, d = o / 128 * 16 + m, t = 16 * a + 8 * u;
+        const u32x4 w = *reinterpret_cast<const u32x4*>(in + (int64_t)o * 16);
 #pragma unroll
-      for (int e = 0; e < 16 / S; ++e) {
-        if constexpr (F8) tile[(t + e) * PITCH + d] = (uint8_t)(w[e / 4] >> (8 * (e % 4)));
-        else *reinterpret_cast<uint16_t*>(&tile[(t + e) * PITCH + 2 * d]) = (uint16_t)(w[e / 2] >> (16 * (e % 2)));
+        for (int e = 0; e < 8; ++e)
+          *reinterpret_cast<uint16_t*>(&tile[(t + e) * PITCH + 2 * d]) = (uint16_t)(w[e / 2] >> (16 * (e % 2)));
       }
     }
   }
