@@ -60,6 +60,9 @@ __device__ __forceinline__ Row row_of(const Params& P, int n, int V) {
   r.m = P.m ? param(P.m, P.f64 & GDN_SAMPLE_F64_MIN_P, n) : P.m1;
   r.k = P.k ? P.k[n] : P.k1;
   r.greedy = !(r.t > 0.0);  // NaN too
+  // at 1e-60 two different fp32 values (2^-149 apart at least) are 1e15 in the exponent apart: nothing below it differs, and
+  // 1 / T times a logit stays a double
+  if (!r.greedy && r.t < 1e-60) r.t = 1e-60;
   if (r.p <= 0.0) r.p = 1e-300;  // the largest alone
   r.by_k = r.k > 0 && r.k < V;
   r.by_p = r.p < 1.0;

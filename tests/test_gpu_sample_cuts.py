@@ -68,3 +68,15 @@ def test_parameters_in_fp64_are_not_rounded(gdn, dev):
     assert gdn.sample_tokens(l, top, t, 0, 1.0, m).tolist() == [1] * 3
     assert gdn.sample_tokens(l, top, one(t), 0, 1.0, m).tolist() == [1] * 3
     assert gdn.sample_tokens(l, top, one(t, torch.float32), 0, 1.0, m).tolist() == [0] * 3
+
+
+@pytest.mark.parametrize("t", [1e-40, 1e-61, 1e-268, 1e-300, 1e-306, 3e-308, 5e-324])
+@pytest.mark.parametrize("base", [-5.0, 0.0, 7.0, -1e30])
+def test_smallest_temperatures(gdn, dev, t, base):
+    """A temperature at which (l - max) / temperature leaves doubles behind: the ties of the maximum share the draw, cut by
+    top_k and top_p as at any other."""
+    l = torch.full((8, 100), base * 2 if base < 0 else base - 1)
+    l[:, [7, 20, 50, 93]] = base
+    u = torch.arange(8) / 8
+    for par in ((t, 0, 0.5, 0.0), (t, 3, 1.0, 0.0), (t, 0, 0.8, 0.1), (t, 30, 0.7, 0.0), (t, 0, 1.0, 0.0)):
+        assert torch.equal(gdn.sample_tokens(l.to(dev), u.to(dev), *par).cpu(), so.sample(l, u.numpy(), *par)), par
