@@ -22,14 +22,15 @@
 // Measured, 24 query and 4 kv heads of 256 (a large read runs at 6.07 TB/s, a large bf16 product at 1374 TFLOP/s), the
 // kernels' medians in us:
 //                                               bytes    prep  split  combine  split's rate
-//   16 slots of 512 to 4096 tokens, e4m3       76 MB     4.2   18.4    3.9     4.1 TB/s
+//   16 slots of 512 to 4096 tokens, e4m3       76 MB     4.3   18.6    4.0     4.1 TB/s
 //   the same, bf16                            152 MB     4.2   27.7    4.2     5.5 TB/s
-//   16 slots of 16384 to 32768 tokens, e4m3   809 MB     5.9  158      6.3     5.1 TB/s
-//   16 slots behind 8192 shared tokens, e4m3   35 MB     6.0   21.0    4.8     164 TFLOP/s
+//   16 slots of 16384 to 32768 tokens, e4m3   809 MB     5.9  157      6.2     5.2 TB/s
+//   16 slots behind 8192 shared tokens, e4m3   35 MB     5.9   21.4    4.8     160 TFLOP/s
 //   64 slots behind 2 x 16384, e4m3           108 MB     7.4   84      5.5     312 TFLOP/s
-// Slots' own tokens are bound by HBM, and where few, by the latency of a workgroup's start and merge (7 us of the 18.4).
+// Slots' own tokens are bound by HBM, and where few, by the latency of a workgroup's start and merge (6 us of the 18.6: 76 MB
+// read are 12.5).
 // A prefix's tiles are bound by the vector instructions around the products (codes widened, the softmax, probabilities
-// split and scaled) at one wave a SIMD.
+// split and scaled) at one wave a SIMD: about 6 us a block of 64 tokens, of which the last case's waves take 13 each.
 #include "gdn_attn.h"
 #include "gdn_device.h"
 #include "gdn_internal.h"

@@ -4,8 +4,9 @@
 // Both are copies: bound by HBM, each value read once and written once.  One workgroup per (64-token cache block,
 // kv head, K or V): a block is what lies together in the cache.  K's 16-byte pieces are one token's and go out as they are;
 // V's lie along the tokens and turn in LDS.  16 prompts of 200 to 1500 tokens (13.6 thousand, 4 heads of 256, bf16 to e4m3
-// and back, 84 MB each way): store 19.7 us (4.2 TB/s), load 17.9 us (4.7 TB/s), where a large copy runs at 4.97 TB/s; 517
-// tokens stored (3.2 MB) and 1541 loaded (9.5 MB): 7.5 and 6.6 us, a launch and a block's latency.
+// and back, 84 MB each way): store 19.6 us (4.3 TB/s), load 17.5 us (4.8 TB/s), where a large copy runs at 4.97 TB/s; the
+// same over a bf16 cache (111 MB each way): 28.6 and 25.2 us (3.9 and 4.4 TB/s: V turns 2 bytes at a time).  517 tokens
+// stored and 1541 loaded, e4m3 (3.2 and 9.5 MB): 7.5 and 6.5 us, bf16: 8.2 and 7.9 us; a launch and a block's latency.
 #include "gdn_internal.h"
 #include "gdn_kv.h"
 

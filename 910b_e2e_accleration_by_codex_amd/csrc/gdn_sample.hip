@@ -18,10 +18,10 @@
 // that a row's sum stays below 2^62).
 //
 // Measured (all filters on; the launches' medians in us: first pass, passes, last pass, draw):
-//    1 x 248320 bf16: 6.5, 8.6, 13.3, 7.4      16 x 248320 bf16: 10.4, 10.5, 15.1, 13.2
-//   64 x 151936 fp32: 15.5, 22.3, 16.1, 15.0, 9.6, 5.9, 18.0, 10.3 (39 MB: a read of it at 6.07 TB/s is 6.4)
+//    1 x 248320 bf16: 6.5, 8.7, 13.5, 7.5      16 x 248320 bf16: 10.3, 10.2, 15.8, 13.4
+//   64 x 151936 fp32: 16.0, 22.3, 16.5, 15.1, 9.8, 5.9, 18.0, 10.2 (39 MB: a read of it at 6.07 TB/s is 6.4)
 // A pass over few rows is a chain of latencies: the histograms' merge and the choice of a bin (3 to 4), the row's load, the
-// LDS counters.  Over many rows the vector instructions bind: 50 to 75 an element, 20 of them its weight in double.
+// LDS counters.  Over many rows the vector instructions bind: 50 to 75 an element, 20 of them its weight.
 #include "gdn_device.h"
 #include "gdn_internal.h"
 

@@ -526,7 +526,8 @@ int gdn_attn_cached(const void* proj, int64_t proj_stride, const float* part, in
  *   out [N] int64.
  *   work: gdn_sample_workspace_bytes(N, V) bytes, 256-byte aligned; its contents need no clearing, one for more rows or
  *     logits holds fewer, and calls that may overlap need one each.
- * Weights and sums are 64-bit, and sums do not depend on an order: the same inputs give the same token.  Replaces the
+ * Weights are good to 4e-10 of their value and summed in 64 bits, and sums do not depend on an order: the same inputs give
+ * the same token.  temperature below 1e-60 is 1e-60 (two different fp32 values are as far apart).  Replaces the
  * argmax over the engine's logits (src/cb_engine.py:170-172).
  */
 int64_t gdn_sample_workspace_bytes(int N, int V);
