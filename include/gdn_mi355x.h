@@ -495,7 +495,7 @@ int gdn_kv_load(const void* k_cache, const void* v_cache, const uint8_t* k_exp, 
  *   gives a zero output; one inside the prefix writes nothing and attends to the prefix alone; one behind the cache
  *   row's end is not written and attends to all of the row.
  *   work: gdn_attn_cached_workspace_bytes(N, nh, nkv, hd, T, P, Tp) bytes, 256-byte aligned (-1: bad sizes).
- * hd in {64, 128, 256}; nh / nkv <= 16; N and P at most 1024.  Scores, softmax and sums are fp32 (scores up to 2^30); the
+ * hd in {64, 128, 256}; nh / nkv <= 16; N and P at most 1024.  Scores, softmax and sums are fp32 (scores up to 2^30 in size); the
  * query enters as two fp16 parts in units of its row's largest value (bf16 caches: as two bf16 parts), the probabilities as
  * two bf16 parts, the output is rounded once; the rotary angle is formed in double.  A graph that captured a call replays it
  * for whatever pos, prefix_len and prefix_of hold then.  Calls that may overlap need a workspace each; its contents need no
